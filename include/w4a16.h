@@ -172,6 +172,84 @@ int w4a16_quantize_pack(const void* W, int w_is_fp32, int64_t N, int64_t K, int6
 int w4a16_gemv(const int32_t* W, const uint16_t* A, const uint16_t* sW, const uint16_t* zW, uint16_t* C,
                int64_t N, int64_t K, void* stream);
 
+/* ---- A key/value cache held in 4 bits, and attention over it ------------------------------------
+ *
+ * No counterpart in the reference, whose users run attention between two of its GEMMs.  The cache is
+ * paged: a page holds page_size consecutive tokens of one sequence, keys and values, for every KV head.
+ * A group of group_size values of one (token, KV head) of K or V is held as s (q - z):
+ *   lo, hi = the group's least and greatest value, each value first clamped to +-65504
+ *   s = fp16(max((hi - lo) / 15, max(|lo|, |hi|) / 96, 2^-14))        (fp32 arithmetic, IEEE divisions)
+ *   z = rint(8 (-lo / s)) / 8                                         (|z| <= 97, so fp16 holds q - z exactly)
+ *   q = clamp(rint(x / s + z), 0, 15)                                 (rint: ties to even)
+ * A group with a NaN has s = z = NaN and reads back as NaN.
+ *
+ * Bytes of one (page, KV head), P = page_size, D = head_dim, G = group_size; P (D + 8 D / G) in all:
+ *   key codes    [P][D/2]           byte j of a token: code of value j in bits 0..3, of j + D/2 in bits 4..7
+ *   value codes  [P/16][D/2][16]    the same byte of token t of 16 at place 4 (t / 4) + {0, 2, 1, 3}[t % 4]
+ *   key scales, key zeros, value scales, value zeros, each fp16 [D/G][P]
+ * and the cache is [pages][kv_heads][those bytes].  Token t of a sequence lies at place t % P of page
+ * block_table[t / P]; its slot is page * P + place. */
+typedef struct w4a16_kv4_cache {
+    void*   data;             /* 16-byte aligned */
+    int64_t pages;
+    int64_t page_size;        /* a multiple of 16, 16..4096 */
+    int64_t kv_heads;         /* 1..1024 */
+    int64_t head_dim;         /* 64 or 128 */
+    int64_t group_size;       /* 64 or 128, dividing head_dim */
+} w4a16_kv4_cache;
+
+/* Bytes of one (page, KV head), 0 where the sizes are not supported. */
+int64_t w4a16_kv4_page_bytes(int64_t page_size, int64_t head_dim, int64_t group_size);
+
+/* Quantise `tokens` tokens' keys and values into their slots (asynchronous, no allocation).
+ * k, v: fp16 (bf16 = 0) or bf16 (bf16 = 1) [tokens, kv_heads, head_dim], head_dim contiguous, the other
+ * strides in elements.  slots: int64 [tokens]; a token whose slot is outside [0, pages * page_size)
+ * is not written (-1 pads a batch).  Two tokens with one slot leave either one's bytes or a mixture.
+ * Returns W4A16_OK, W4A16_ERR_INVALID (message via w4a16_last_error) or W4A16_ERR_HIP. */
+int w4a16_kv4_write(const w4a16_kv4_cache* cache, const void* k, const void* v, int bf16, int64_t tokens,
+                    int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride,
+                    int64_t v_head_stride, const int64_t* slots, void* stream);
+
+/* Read tokens back: k, v [tokens, kv_heads, head_dim] contiguous, fp16 or bf16, the exact s (q - z)
+ * rounded once.  A slot outside [0, pages * page_size) gives zeros.  Asynchronous, no allocation. */
+int w4a16_kv4_read(const w4a16_kv4_cache* cache, const int64_t* slots, int64_t tokens, int bf16,
+                   void* k, void* v, void* stream);
+
+/* Attention of a batch's queries over the cache:
+ *   out[i, h] = sum_t p_t v_t / sum_t p_t,   p_t = exp(scale * q[i, h] . k_t)
+ * over the tokens t that query i of its sequence sees.  Sequence b holds seq_lens[b] tokens, its m
+ * queries q_start[b] .. q_start[b + 1] - 1 are the last m of them: query i stands at
+ * pos = seq_lens[b] - m + i and sees t < seq_lens[b], with `causal` only t <= pos, and with
+ * window > 0 only t > pos - window.  Query head h reads KV head h / (heads / kv_heads).  A query that
+ * sees nothing gives zeros (lse -inf).  Tokens on a table entry outside [0, pages) are not seen, and
+ * lengths and starts are clamped to what the table and q hold, so no index reads out of bounds. */
+typedef struct w4a16_kv4_attention_args {
+    const void* q;            /* fp16 or bf16 [tokens, heads, head_dim], head_dim contiguous */
+    void*   out;              /* the same type, contiguous */
+    float*  lse;              /* NULL, or fp32 [tokens, heads]: log sum_t p_t */
+    int64_t q_token_stride, q_head_stride;   /* in elements */
+    int64_t tokens, heads, batch;
+    const int32_t* block_table;              /* [batch, table_width], rows table_stride apart */
+    int64_t table_width, table_stride;
+    const int32_t* seq_lens;  /* [batch] */
+    const int32_t* q_start;   /* [batch + 1], or NULL: one query per sequence (tokens == batch) */
+    int64_t max_q;            /* queries of the longest sequence (selects the kernel; results hold for any value >= 1) */
+    int64_t window;           /* 0: none */
+    float   scale;            /* positive */
+    int32_t bf16;
+    int32_t causal;
+} w4a16_kv4_attention_args;
+
+/* Bytes of device memory that w4a16_kv4_attention needs beside its arguments (0 if none); pure host
+ * code.  -1 where the arguments are invalid (message via w4a16_last_error). */
+int64_t w4a16_kv4_attention_workspace(const w4a16_kv4_cache* cache, const w4a16_kv4_attention_args* args,
+                                      const w4a16_device_limits* lim);
+
+/* workspace: 16-byte aligned, of at least those bytes (no initialisation); NULL where 0.
+ * Asynchronous, no allocation, no host synchronisation: it may be captured into a graph. */
+int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4_attention_args* args,
+                        const w4a16_device_limits* lim, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* Query the limits of HIP device `device` (cached per device, thread-safe). */
 int w4a16_query_device(int device, w4a16_device_limits* lim);
 

@@ -8,6 +8,7 @@ Outputs (next to this file, git-ignored, shipped to the GPU box with the tree):
   w4a16_opt<EXT_SUFFIX>        host-compiler (g++) PyTorch extension linking libw4a16_hip.so
                                through an $ORIGIN rpath; import it as `w4a16_opt`.
   w4a16_ext<EXT_SUFFIX>        the same for the baseline GEMV module `w4a16_ext`.
+  w4a16_kv<EXT_SUFFIX>         the same for the 4-bit key/value cache module `w4a16_kv`.
   libw4a16_bwprobe.so          bandwidth probes of measure_bw.py.
   libw4a16_hip_stamps.so       the same library built with -DW4A16_WAVE_STAMPS: the decode ring
                                kernel records per-wave timestamps (wave_timeline.py); never
@@ -30,6 +31,7 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 LIB = os.path.join(HERE, "libw4a16_hip.so")
 EXT = os.path.join(HERE, "w4a16_opt" + sysconfig.get_config_var("EXT_SUFFIX"))
 EXT_GEMV = os.path.join(HERE, "w4a16_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
+EXT_KV = os.path.join(HERE, "w4a16_kv" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 # gfx950 only; packed-fp32 VALU ops disabled for all device code (-packed-fp32-ops).
 HIPCC_FLAGS = [
@@ -62,6 +64,8 @@ SOURCES = [
                                 "-mllvm", "-amdgpu-kernarg-preload-count=16"]),
     ("w4a16_quantize.hip", []),
     ("w4a16_gemv.hip", ["-mllvm", "-amdgpu-kernarg-preload-count=16"]),
+    ("w4a16_kv4.hip", []),
+    ("w4a16_kv4_attn.hip", []),
     ("w4a16_plan.cpp", []),
 ]
 
@@ -153,9 +157,10 @@ def main(argv=None) -> int:
     a = ap.parse_args(argv)
     build_lib(with_stamps=not a.lib)
     if not a.lib:
-        with concurrent.futures.ThreadPoolExecutor(max_workers=4) as pool:
+        with concurrent.futures.ThreadPoolExecutor(max_workers=5) as pool:
             jobs = [pool.submit(build_stamps), pool.submit(build_probe), pool.submit(build_ext),
-                    pool.submit(build_ext, "w4a16_ext", "w4a16_ext_torch.cpp", EXT_GEMV)]
+                    pool.submit(build_ext, "w4a16_ext", "w4a16_ext_torch.cpp", EXT_GEMV),
+                    pool.submit(build_ext, "w4a16_kv", "w4a16_kv_torch.cpp", EXT_KV)]
             for job in jobs:
                 job.result()
     return 0

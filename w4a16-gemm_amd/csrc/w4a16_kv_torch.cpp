@@ -1,0 +1,162 @@
+// PyTorch-ROCm binding: module `w4a16_kv`, a key/value cache held in 4 bits and attention over it.
+//
+// The tensor-level half of the kv4 entry points of include/w4a16.h: checks, device guard, the current stream,
+// outputs and workspace.  A cache is one uint8 tensor [pages, kv_heads, P (D + 8 D / G)]: the page size P
+// follows from its last size, the head size D and the group size G.
+//
+// Compiled by the host compiler (no hipify, no device code).
+#include <torch/extension.h>
+
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+
+#include <algorithm>
+#include <cmath>
+#include <optional>
+#include <tuple>
+
+#include "w4a16.h"
+
+namespace {
+
+int is_bf16(at::ScalarType t, const char* what) {
+    TORCH_CHECK(t == torch::kHalf || t == torch::kBFloat16, what, " must be fp16 or bf16");
+    return t == torch::kBFloat16;
+}
+
+w4a16_kv4_cache cache_of(const torch::Tensor& cache, int64_t head_dim, int64_t group_size) {
+    TORCH_CHECK(cache.dtype() == torch::kUInt8, "cache must be uint8");
+    TORCH_CHECK(cache.dim() == 3, "cache must be [pages, kv_heads, bytes of a page and head]");
+    TORCH_CHECK(cache.is_contiguous(), "cache must be contiguous");
+    const int64_t unit = w4a16_kv4_page_bytes(16, head_dim, group_size);
+    TORCH_CHECK(unit > 0, "unsupported head and group size (", head_dim, ", ", group_size, "), supported: (64, 64), (128, 64), (128, 128)");
+    TORCH_CHECK(cache.size(2) > 0 && cache.size(2) % unit == 0, "cache's last size is not that of whole tiles of 16 tokens of head size ",
+                head_dim, " in groups of ", group_size);
+    return w4a16_kv4_cache{cache.data_ptr(), cache.size(0), 16 * (cache.size(2) / unit), cache.size(1), head_dim, group_size};
+}
+
+void check_slots(const torch::Tensor& slots, const torch::Tensor& cache) {
+    TORCH_CHECK(slots.dtype() == torch::kInt64, "slots must be int64");
+    TORCH_CHECK(slots.dim() == 1, "slots must be [tokens]");
+    TORCH_CHECK(slots.is_contiguous(), "contiguous only");
+    TORCH_CHECK(slots.device() == cache.device(), "all tensors must be on the same device");
+}
+
+void* stream_of(const torch::Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
+
+}  // namespace
+
+torch::Tensor kv4_cache(int64_t pages, int64_t page_size, int64_t kv_heads, int64_t head_dim, int64_t group_size, py::object device) {
+    const int64_t bytes = w4a16_kv4_page_bytes(page_size, head_dim, group_size);
+    TORCH_CHECK(bytes > 0, "kv4_cache: unsupported sizes: pages of 16..4096 tokens (a multiple of 16), (head, group) sizes (64, 64), "
+                           "(128, 64), (128, 128)");
+    TORCH_CHECK(pages >= 0 && kv_heads >= 1, "kv4_cache: pages must be at least 0 and kv_heads at least 1");
+    const auto dev = py::module_::import("torch").attr("device")(device).cast<torch::Device>();      // a name or a device
+    return torch::zeros({pages, kv_heads, bytes}, torch::TensorOptions().dtype(torch::kUInt8).device(dev));
+}
+
+void kv4_write(torch::Tensor cache, torch::Tensor k, torch::Tensor v, torch::Tensor slots, int64_t group_size) {
+    TORCH_CHECK(cache.is_cuda() && k.is_cuda() && v.is_cuda() && slots.is_cuda(), "all tensors must be CUDA");
+    TORCH_CHECK(k.dim() == 3 && v.dim() == 3, "k and v must be [tokens, kv_heads, head_dim]");
+    TORCH_CHECK(k.sizes() == v.sizes(), "k and v must have the same sizes");
+    const int bf16 = is_bf16(k.scalar_type(), "k");
+    TORCH_CHECK(v.scalar_type() == k.scalar_type(), "k and v must have the same dtype");
+    const w4a16_kv4_cache c = cache_of(cache, k.size(2), group_size);
+    TORCH_CHECK(k.size(1) == c.kv_heads, "k and v have ", k.size(1), " heads, the cache ", c.kv_heads);
+    TORCH_CHECK(k.numel() == 0 || (k.stride(2) == 1 && v.stride(2) == 1), "k and v must be contiguous in the head dimension");
+    check_slots(slots, cache);
+    TORCH_CHECK(slots.size(0) == k.size(0), "slots must be [tokens]");
+    TORCH_CHECK(k.device() == cache.device() && v.device() == cache.device(), "all tensors must be on the same device");
+    const c10::DeviceGuard guard(cache.device());
+    const int rc = w4a16_kv4_write(&c, k.data_ptr(), v.data_ptr(), bf16, k.size(0), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                                   slots.data_ptr<int64_t>(), stream_of(cache));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+}
+
+std::tuple<torch::Tensor, torch::Tensor> kv4_read(torch::Tensor cache, torch::Tensor slots, int64_t head_dim, int64_t group_size,
+                                                  at::ScalarType dtype) {
+    TORCH_CHECK(cache.is_cuda() && slots.is_cuda(), "all tensors must be CUDA");
+    const int bf16 = is_bf16(dtype, "dtype");
+    const w4a16_kv4_cache c = cache_of(cache, head_dim, group_size);
+    check_slots(slots, cache);
+    const c10::DeviceGuard guard(cache.device());
+    const auto opts = cache.options().dtype(dtype);
+    torch::Tensor k = torch::empty({slots.size(0), c.kv_heads, head_dim}, opts), v = torch::empty_like(k);
+    const int rc = w4a16_kv4_read(&c, slots.data_ptr<int64_t>(), slots.size(0), bf16, k.data_ptr(), v.data_ptr(), stream_of(cache));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+    return {k, v};
+}
+
+py::object kv4_attention(torch::Tensor q, torch::Tensor cache, torch::Tensor block_table, torch::Tensor seq_lens, int64_t group_size,
+                         std::optional<torch::Tensor> q_start, int64_t max_q, std::optional<double> scale, bool causal, int64_t window,
+                         bool return_lse) {
+    TORCH_CHECK(q.is_cuda() && cache.is_cuda() && block_table.is_cuda() && seq_lens.is_cuda() && (!q_start || q_start->is_cuda()),
+                "all tensors must be CUDA");
+    TORCH_CHECK(q.dim() == 3, "q must be [tokens, heads, head_dim]");
+    const int bf16 = is_bf16(q.scalar_type(), "q");
+    const w4a16_kv4_cache c = cache_of(cache, q.size(2), group_size);
+    TORCH_CHECK(q.numel() == 0 || q.stride(2) == 1, "q must be contiguous in the head dimension");
+    TORCH_CHECK(q.size(1) > 0 && q.size(1) % c.kv_heads == 0, "q has ", q.size(1), " heads, not a multiple of the cache's ", c.kv_heads);
+    TORCH_CHECK(block_table.dtype() == torch::kInt32 && seq_lens.dtype() == torch::kInt32 && (!q_start || q_start->dtype() == torch::kInt32),
+                "block_table, seq_lens and q_start must be int32");
+    TORCH_CHECK(block_table.dim() == 2 && seq_lens.dim() == 1 && block_table.size(0) == seq_lens.size(0),
+                "block_table must be [batch, pages of the longest sequence], seq_lens [batch]");
+    const int64_t batch = seq_lens.size(0);
+    TORCH_CHECK(block_table.numel() == 0 || block_table.stride(1) == 1, "block_table's rows must be contiguous");
+    TORCH_CHECK(seq_lens.is_contiguous() && (!q_start || q_start->is_contiguous()), "contiguous only");
+    TORCH_CHECK(!q_start || (q_start->dim() == 1 && q_start->size(0) == batch + 1), "q_start must be [batch + 1]");
+    TORCH_CHECK(q_start || q.size(0) == batch, "without q_start there is one query per sequence: q has ", q.size(0), " tokens, the batch ", batch);
+    TORCH_CHECK(max_q >= 0, "max_q must not be negative");
+    TORCH_CHECK(window >= 0, "window must not be negative");
+    TORCH_CHECK(cache.device() == q.device() && block_table.device() == q.device() && seq_lens.device() == q.device() &&
+                    (!q_start || q_start->device() == q.device()),
+                "all tensors must be on the same device");
+    const double s = scale ? *scale : 1.0 / std::sqrt((double)q.size(2));
+    TORCH_CHECK(s > 0 && std::isfinite((float)s), "scale must be positive and finite");
+
+    const c10::DeviceGuard guard(q.device());
+    w4a16_device_limits lim;
+    TORCH_CHECK(w4a16_query_device(q.device().index(), &lim) == W4A16_OK, "kv4_attention: device query failed: ", w4a16_last_error());
+    torch::Tensor out = torch::empty({q.size(0), q.size(1), q.size(2)}, q.options()), lse;
+    if (return_lse) lse = torch::empty({q.size(0), q.size(1)}, q.options().dtype(torch::kFloat));
+    w4a16_kv4_attention_args a{};
+    a.q = q.data_ptr();
+    a.out = out.data_ptr();
+    a.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+    a.q_token_stride = q.stride(0);
+    a.q_head_stride = q.stride(1);
+    a.tokens = q.size(0);
+    a.heads = q.size(1);
+    a.batch = batch;
+    a.block_table = block_table.data_ptr<int32_t>();
+    a.table_width = block_table.size(1);
+    a.table_stride = block_table.stride(0);
+    a.seq_lens = seq_lens.data_ptr<int32_t>();
+    a.q_start = q_start ? q_start->data_ptr<int32_t>() : nullptr;
+    a.max_q = !q_start ? 1 : std::max<int64_t>(1, max_q ? std::min(max_q, a.tokens) : a.tokens);
+    a.window = window;
+    a.scale = (float)s;
+    a.bf16 = bf16;
+    a.causal = causal;
+    const int64_t bytes = w4a16_kv4_attention_workspace(&c, &a, &lim);
+    TORCH_CHECK(bytes >= 0, w4a16_last_error());
+    torch::Tensor ws;
+    if (bytes) ws = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
+    const int rc = w4a16_kv4_attention(&c, &a, &lim, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q));
+    TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
+    return return_lse ? py::cast(std::make_tuple(out, lse)) : py::cast(out);
+}
+
+PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.def("kv4_cache", &kv4_cache, "A zeroed 4-bit key/value cache: uint8 [pages, kv_heads, bytes of a page and head]", py::arg("pages"),
+          py::arg("page_size"), py::arg("kv_heads"), py::arg("head_dim"), py::arg("group_size"),
+          py::arg("device") = "cuda");
+    m.def("kv4_write", &kv4_write, "Quantise k, v [tokens, kv_heads, head_dim] into the cache at slots [tokens] (page * page_size + place)",
+          py::arg("cache"), py::arg("k"), py::arg("v"), py::arg("slots"), py::arg("group_size"));
+    m.def("kv4_read", &kv4_read, "The keys and values that the cache holds at slots [tokens]: (k, v) [tokens, kv_heads, head_dim]",
+          py::arg("cache"), py::arg("slots"), py::arg("head_dim"), py::arg("group_size"), py::arg("dtype") = torch::kHalf);
+    m.def("kv4_attention", &kv4_attention,
+          "Attention of q [tokens, heads, head_dim] over the cache: out, or (out, lse) with return_lse", py::arg("q"), py::arg("cache"),
+          py::arg("block_table"), py::arg("seq_lens"), py::arg("group_size"), py::arg("q_start") = py::none(), py::arg("max_q") = 0,
+          py::arg("scale") = py::none(), py::arg("causal") = true, py::arg("window") = 0, py::arg("return_lse") = false);
+}
