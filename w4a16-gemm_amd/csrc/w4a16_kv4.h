@@ -78,6 +78,7 @@ struct Kv4Attn {
     int window;                              // 0: none
     float scale2;                            // scale * log2(e)
     int bf16, causal;
+    int q_wide;                              // q's rows can be read 16 bytes at a time
 };
 
 // What one sequence asks: queries first .. first + count - 1, keys 0 .. len - 1.

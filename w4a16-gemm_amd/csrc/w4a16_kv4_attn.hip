@@ -1,10 +1,22 @@
 // Attention over the 4-bit key/value cache (include/w4a16.h has the format and what is computed).
 #include <math.h>
 
+#include <algorithm>
+
 #include "w4a16_internal.h"
 #include "w4a16_kv4.h"
 
 namespace w4a16 {
+
+// Two neighbouring values of a row's result, and its lse: top and sum are the row's largest score (base 2) and the
+// sum of 2^(score - top).  A row that sees nothing (sum 0) gives zeros and -inf; a NaN stays one.
+template <int D>
+__device__ __forceinline__ void kv4_finish(const Kv4Attn& a, int64_t row, int d, float top, float sum, float v0, float v1) {
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    *reinterpret_cast<uint32_t*>(a.out + row * D + d) =
+        (uint32_t)store16(v0 * inv, a.bf16) | ((uint32_t)store16(v1 * inv, a.bf16) << 16);
+    if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
+}
 
 // One wave per (query, query head).  Keys go by in tiles of 64: lane t takes the score of key t, the tile's
 // probabilities pass through LDS, and lane d adds up values d and d + D/2.
@@ -92,11 +104,455 @@ kv4_attention_kernel(Kv4Attn a) {
     }
 }
 
+// ------------------------------------------------------------------------------------------------
+// Few rows (single tokens, drafts): kv4_token_kernel
+
+typedef int i4v __attribute__((ext_vector_type(4)));
+
+// All-lane results over the 16 lanes of a row: neighbours, pairs, quads, halves.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(int, v)));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+#define W4A16_OVER_ROW(v, op)              \
+    do {                                   \
+        v = op(v, dpp<kXor1>(v));          \
+        v = op(v, dpp<kXor2>(v));          \
+        v = op(v, dpp<kHalfMirror>(v));    \
+        v = op(v, dpp<kMirror>(v));        \
+    } while (0)
+__device__ __forceinline__ float add(float a, float b) { return a + b; }
+
+__device__ __forceinline__ void wave_lds_order() {           // a wave's own LDS operations stay in order
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Fixed point in signed digits of 8 bits, byte i of the result digit i: three of |v| <= 2^22 (byte 3 is 0), four of
+// 0 <= v <= 2^30; and sums of digits times what they multiply, put together again.
+__device__ __forceinline__ uint32_t digits3(int v) { return (uint32_t)(v + 0x00808080) ^ 0x00808080u; }
+__device__ __forceinline__ uint32_t digits4(int v) { return ((uint32_t)v + 0x80808080u) ^ 0x80808080u; }
+__device__ __forceinline__ float of_digits3(int d0, int d1, int d2) { return fmaf((float)d2, 65536.f, (float)((d1 << 8) + d0)); }
+__device__ __forceinline__ float of_digits4(int d0, int d1, int d2, int d3) {
+    return fmaf((float)((d3 << 8) + d2), 65536.f, (float)((d1 << 8) + d0));
+}
+
+// Keys and values of 64 tokens in flight, for lane (kb, n) = (lane / 16, lane % 16).
+template <int D, int NG>
+struct KvTile {
+    u4 k[4];                                 // 16 bytes of the row of token 16 r + n
+    u4 v[D / 32];                            // tokens 16 kb .. + 15 of byte n + 16 i
+    uint16_t side[4][NG];                    // of token 16 kb + n
+    bool there;                              // the page of tokens 16 kb .. + 15 is in the cache
+};
+
+// One workgroup takes one KV head of one sequence and a share of its tiles of 64 keys, a wave one tile at a time;
+// 4 NT rows (query, query head) at once.  Both products run on v_mfma_i32_16x16x64_i8: the codes are its operand as
+// they lie in the cache (one mask, for the upper codes one shift), the other operand is a fixed-point number in
+// digits, which fill the rows that four query heads leave of the 16: row 4 r + i is digit i of row r.
+//   scores  x = rs s_t (sum_d q_d c_td - z_t sum_d q_d)     q to 2^-22 of the power of two above its row's largest
+//   values  o = sum_t (p_t s_t) (8 c_td - 8 z_t) / 8         p s to 2^-30 of the power of two above the tile's largest s
+// The integer sums are exact, those of 8 z_t (in two digits, one more column of the product) among them, and are taken
+// off digit by digit: a value that is 0 weighs nothing however large p is.  The digits come together in fp32.  Per 64 keys a wave issues about 300 vector
+// instructions for 8.7 KB, under a third of the time that HBM takes to bring them.
+template <int D, int G, int NT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES)
+kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
+                 float* __restrict__ part_o) {
+    constexpr int NG = D / G;                                // groups of a token: of lower and of upper codes where 2
+    constexpr int NV = D / 32;                               // 16-byte pieces per lane of a value tile
+    constexpr int kSide = NG * (64 * 8 + 128), kDigits = NT * NG * 1024;
+    constexpr int kLoop = WAVES * (kSide + kDigits), kJoin = WAVES * 4 * NT * (D + 2) * 4;
+    __shared__ __align__(16) uint8_t lds[kLoop > kJoin ? kLoop : kJoin];
+    const int lane = threadIdx.x & 63, kb = lane >> 4, n = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    uint8_t* const side = lds + wave * (kSide + kDigits);
+    uint8_t* const dig = side + kSide;
+    const int h = blockIdx.x % a.c.H, split = blockIdx.x / a.c.H, b = blockIdx.y;
+    const Kv4Seq s = kv4_seq(a, b);
+    const int rows = s.count * a.rep, base = s.len - s.count, groups = a.c.P >> 4;
+    const int* const table = a.table + b * a.table_stride;
+    const uint32_t quad_a = lane & 1 ? 0x03070105u : 0x06020400u;   // selectors of the 4 x 4 byte transpose below
+    const uint32_t quad_b = lane & 2 ? 0x03070206u : 0x05010400u;
+
+    for (int row0 = 0; row0 < rows; row0 += 4 * NT) {
+        const int first = row0 / a.rep, last = (min(row0 + 4 * NT, rows) - 1) / a.rep;
+        const int kmax = a.causal ? max(0, min(base + last + 1, s.len)) : s.len;
+        const int kmin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
+        const int tile0 = kmin >> 6, tiles = a.c.pages > 0 ? max(0, ((kmax + 63) >> 6) - tile0) : 0;
+        const int per = max(WAVES, (tiles + splits - 1) / splits), parts = max(1, (tiles + per - 1) / per);
+        if (split >= parts) continue;
+        // keys that every row sees: no masks where a tile lies within
+        const int sure_end = a.causal ? min(base + first + 1, s.len) : s.len;
+        const int sure_begin = a.window > 0 ? max(0, base + last - a.window + 1) : 0;
+
+        // The rows' queries as digits, in the order of the cache's bytes
+        i4v qd[NT][D / 64];
+        float rs[NT], qsum[NT][NG];
+        int begin[NT], end[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int r = row0 + 4 * t + (n >> 2);
+            float x[D / 64][16];
+            uint32_t top = 0;
+            if (r < rows) {
+                const uint16_t* src = a.q + (int64_t)(s.first + r / a.rep) * a.q_token + (int64_t)(h * a.rep + r % a.rep) * a.q_head + 16 * kb;
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i) {
+                    if (a.q_wide) {
+                        const u4 lo = *reinterpret_cast<const u4*>(src + 64 * i), hi = *reinterpret_cast<const u4*>(src + 64 * i + 8);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const uint32_t w0 = lo[j], w1 = hi[j];
+                            x[i][2 * j] = load16(w0 & 0xFFFF, a.bf16);
+                            x[i][2 * j + 1] = load16(w0 >> 16, a.bf16);
+                            x[i][8 + 2 * j] = load16(w1 & 0xFFFF, a.bf16);
+                            x[i][8 + 2 * j + 1] = load16(w1 >> 16, a.bf16);
+                        }
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) x[i][j] = load16(src[64 * i + j], a.bf16);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) x[i][j] = 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) top = max(top, __builtin_bit_cast(uint32_t, x[i][j]) & 0x7FFFFFFFu);
+            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+            const bool finite = top < 0x7F800000u;
+            const int e = finite ? __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) : 0;   // |x| < 2^e
+            int sums[D / 64];
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                int sum = 0;
+                uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const int v = finite ? (int)rintf(ldexpf(x[i][j], 22 - e)) : 0;
+                    sum += v;
+                    w[j >> 2] |= ((digits3(v) >> (8 * (n & 3))) & 0xFFu) << (8 * (j & 3));
+                }
+                qd[t][i] = i4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
+                sum += __shfl_xor(sum, 16, 64);
+                sums[i] = sum + __shfl_xor(sum, 32, 64);
+            }
+            // from here on lane (kb, n) stands for row kb
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const int sum = NG == 2 || D == 64 ? sums[g] : sums[0] + sums[D / 64 - 1];
+                qsum[t][g] = (float)__shfl(sum, 4 * kb, 64);
+            }
+            rs[t] = __shfl(finite ? ldexpf(a.scale2, e - 22) : NAN, 4 * kb, 64);
+            const int mine = row0 + 4 * t + kb, pos = base + mine / a.rep;
+            end[t] = mine < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
+            begin[t] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        }
+
+        float m[NT], l[NT], nan[NT][NG], o[NT][2][NV];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) nan[t][g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) o[t][0][i] = o[t][1][i] = 0.f;
+        }
+
+        // A tile's page and place in it for the lane's 16 tokens: the table entry comes one tile ahead of the tile
+        auto entry = [&](int tile) {
+            const int group = tile * 4 + kb;
+            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
+            return group * 16 < kmax ? table[at] : -1;
+        };
+        auto load = [&](int tile, int page, KvTile<D, NG>& x) {
+            const int group = tile * 4 + kb;
+            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
+            const int place = (group - at * groups) * 16;
+            x.there = (uint32_t)page < (uint32_t)a.c.pages;
+            const int pg = x.there ? page : 0;
+            const uint8_t* mine = a.c.head(pg, h);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint8_t* row = a.c.head(__builtin_amdgcn_readlane(pg, 16 * r), h) + kv4_key_row<D>(__builtin_amdgcn_readlane(place, 16 * r));
+                x.k[r] = *reinterpret_cast<const u4*>(row + n * (D / 2) + 16 * (D == 128 ? kb : kb & 1));
+            }
+            const uint8_t* vals = mine + kv4_value_tile<D>(a.c.P, place) + n * 16;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) x.v[i] = *reinterpret_cast<const u4*>(vals + 256 * i);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    x.side[w][g] = *reinterpret_cast<const uint16_t*>(mine + kv4_side<D, G>(a.c.P, w, g, place + n));
+        };
+
+        const int stop = tile0 + min(tiles, (split + 1) * per);
+        int tile = tile0 + split * per + wave;
+        KvTile<D, NG> x;
+        int next_page = -1;
+        if (tile < stop) {
+            load(tile, entry(tile), x);
+            if (tile + WAVES < stop) next_page = entry(tile + WAVES);
+        }
+        for (; tile < stop; tile += WAVES) {
+            const KvTile<D, NG> c = x;
+            if (tile + WAVES < stop) {
+                load(tile + WAVES, next_page, x);
+                if (tile + 2 * WAVES < stop) next_page = entry(tile + 2 * WAVES);
+            }
+            // scales and zeros through LDS, nothing for tokens that no row sees; the largest value scale
+            const bool live = c.there && tile * 64 + lane < kmax;
+            uint32_t big = 0;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                u2 w = u2{(uint32_t)c.side[kKeyScale][g] | ((uint32_t)c.side[kKeyZero][g] << 16), c.side[kValueScale][g]};
+                int z = (int)(half_bits(c.side[kValueZero][g]) * 8.f);
+                if (!live) {
+                    w = u2{0, 0};
+                    z = 0;
+                }
+                *reinterpret_cast<u2*>(side + (g * 64 + lane) * 8) = w;
+                uint8_t* const zb = side + NG * 512 + g * 128 + kb * 32 + kv4_place(n);
+                zb[0] = (uint8_t)(z & 15);
+                zb[16] = (uint8_t)(z >> 4);
+                big = max(big, min(w.y, 0x7BFFu));
+            }
+            {
+                int v = (int)big;
+                W4A16_OVER_ROW(v, max);
+                big = (uint32_t)max(max(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+                                    max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+            }
+            // every value scale is under 2^(ev - 14), p s in units of 2^(ev - 44) under 2^30
+            const int ev = (int)(big >> 10);
+            const float unit = __builtin_bit_cast(float, (uint32_t)(127 + 44 - ev) << 23);
+            const float back = __builtin_bit_cast(float, (uint32_t)(127 - 47 + ev) << 23);
+            const bool whole = __all(live) && tile * 64 + 64 <= sure_end && tile * 64 >= sure_begin;
+            wave_lds_order();
+
+            float sc[NT][4], sv[4][NG];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                float sk[NG], zk[NG];
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const u2 w = *reinterpret_cast<const u2*>(side + (g * 64 + 16 * r + n) * 8);
+                    const uint32_t w0 = w.x, w1 = w.y;
+                    sk[g] = half_bits(w0 & 0xFFFF);
+                    zk[g] = half_bits(w0 >> 16);
+                    sv[r][g] = half_bits(w1 & 0xFFFF);
+                }
+                const u4 w = c.k[r];
+                i4v code[D / 64];
+                if constexpr (D == 128) {
+                    code[0] = __builtin_bit_cast(i4v, w & 0x0F0F0F0Fu);
+                    code[1] = __builtin_bit_cast(i4v, (w >> 4) & 0x0F0F0F0Fu);
+                } else {
+                    code[0] = __builtin_bit_cast(i4v, (w >> (kb >= 2 ? 4u : 0u)) & 0x0F0F0F0Fu);
+                }
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    i4v dot[NG];
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) dot[g] = i4v{0, 0, 0, 0};
+#pragma unroll
+                    for (int i = 0; i < D / 64; ++i)
+                        dot[NG == 2 ? i : 0] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qd[t][i], code[i], dot[NG == 2 ? i : 0], 0, 0, 0);
+                    float y = 0.f;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) y += fmaf(-zk[g], qsum[t][g], of_digits3(dot[g][0], dot[g][1], dot[g][2])) * sk[g];
+                    sc[t][r] = y * rs[t];
+                }
+            }
+            i4v pd[NT][NG];
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                bool see[4] = {true, true, true, true};
+                if (!whole) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int at = tile * 64 + 16 * r + n;
+                        see[r] = __builtin_amdgcn_readlane((int)c.there, 16 * r) && at < end[t] && at >= begin[t];
+                        if (!see[r]) sc[t][r] = -INFINITY;
+                    }
+                }
+                float top = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]));
+                W4A16_OVER_ROW(top, fmaxf);
+                const float next = fmaxf(m[t], top), safe = next == -INFINITY ? 0.f : next;
+                const float keep = __builtin_amdgcn_exp2f(m[t] - safe);
+                m[t] = next;
+                l[t] *= keep;
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    o[t][0][i] *= keep;
+                    o[t][1][i] *= keep;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const float p = __builtin_amdgcn_exp2f(sc[t][r] - safe);
+                    l[t] += p;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        float ps = p * sv[r][g];
+                        if (!whole && !see[r]) ps = 0.f;            // a token that another row sees may hold NaN
+                        nan[t][g] = fmaf(ps, 0.f, nan[t][g]);
+                        // four neighbouring lanes exchange bytes so that lane i of them holds digit i of their tokens
+                        uint32_t d = digits4((int)(ps * unit));
+                        d = __builtin_amdgcn_perm((uint32_t)dpp<kXor1>((int)d), d, quad_a);
+                        d = __builtin_amdgcn_perm((uint32_t)dpp<kXor2>((int)d), d, quad_b);
+                        *reinterpret_cast<uint32_t*>(dig + (t * NG + g) * 1024 + r * 256 + (4 * kb + (n & 3)) * 16 + (n & 12)) = d;
+                    }
+                }
+            }
+            wave_lds_order();
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) pd[t][g] = *reinterpret_cast<const i4v*>(dig + (t * NG + g) * 1024 + kb * 256 + n * 16);
+            // sums of digits times 8 z: even columns hold those of its low digit, odd ones of its high
+            int cz[NT][NG][4];
+            const int low = n & 1 ? 16 : 1, high = n & 1 ? 1 : 16;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) {
+                const i4v zb = *reinterpret_cast<const i4v*>(side + NG * 512 + g * 128 + kb * 32 + (n & 1) * 16);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const i4v none = {0, 0, 0, 0};
+                    const i4v y = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][g], zb, none, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) cz[t][g][i] = __mul24(y[i], low) + __mul24(dpp<kXor1>(y[i]), high);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const u4 w = c.v[i];
+                const i4v lo = __builtin_bit_cast(i4v, w & 0x0F0F0F0Fu), hi = __builtin_bit_cast(i4v, (w >> 4) & 0x0F0F0F0Fu);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const i4v none = {0, 0, 0, 0};
+                    const i4v y0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][0], lo, none, 0, 0, 0);
+                    const i4v y1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][NG - 1], hi, none, 0, 0, 0);
+                    int e0[4], e1[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        e0[j] = (y0[j] << 3) - cz[t][0][j];
+                        e1[j] = (y1[j] << 3) - cz[t][NG - 1][j];
+                    }
+                    o[t][0][i] = fmaf(of_digits4(e0[0], e0[1], e0[2], e0[3]), back, o[t][0][i]);
+                    o[t][1][i] = fmaf(of_digits4(e1[0], e1[1], e1[2], e1[3]), back, o[t][1][i]);
+                }
+            }
+        }
+
+        // The waves' shares come together in LDS
+        float* const jm = reinterpret_cast<float*>(lds);
+        float* const jl = jm + WAVES * 4 * NT;
+        float* const jo = jl + WAVES * 4 * NT;
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float sum = l[t];
+            W4A16_OVER_ROW(sum, add);
+#pragma unroll
+            for (int g = 0; g < NG; ++g) W4A16_OVER_ROW(nan[t][g], add);
+            const int r = wave * 4 * NT + 4 * t + kb;
+            if (n == 0) {
+                jm[r] = m[t];
+                jl[r] = sum;
+            }
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                jo[r * D + n + 16 * i] = o[t][0][i] + nan[t][0];
+                jo[r * D + D / 2 + n + 16 * i] = o[t][1][i] + nan[t][NG - 1];
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 4 * NT * (D / 2); i += 64 * WAVES) {
+            const int r = i / (D / 2), d = i % (D / 2) * 2, mine = row0 + r;
+            if (mine >= rows) continue;
+            float top = jm[r];
+#pragma unroll
+            for (int w = 1; w < WAVES; ++w) top = fmaxf(top, jm[w * 4 * NT + r]);
+            const float safe = top == -INFINITY ? 0.f : top;
+            float sum = 0.f, v0 = 0.f, v1 = 0.f;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                const float f = __builtin_amdgcn_exp2f(jm[w * 4 * NT + r] - safe);
+                const float2 y = *reinterpret_cast<const float2*>(jo + (w * 4 * NT + r) * D + d);
+                sum = fmaf(f, jl[w * 4 * NT + r], sum);
+                v0 = fmaf(f, y.x, v0);
+                v1 = fmaf(f, y.y, v1);
+            }
+            const int64_t row = (int64_t)(s.first + mine / a.rep) * a.heads + h * a.rep + mine % a.rep;
+            if (parts == 1) {
+                kv4_finish<D>(a, row, d, top, sum, v0, v1);
+                if (used && d == 0) used[row] = 1;
+            } else {
+                const int64_t at = row * splits + split;
+                *reinterpret_cast<float2*>(part_o + at * D + d) = float2{v0, v1};
+                if (d == 0) {
+                    part_ml[at] = float2{top, sum};
+                    if (split == 0) used[row] = parts;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// Joins the shares of one row (used[row] of them, each of its own part of the keys): one workgroup per row.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv4_join_kernel(Kv4Attn a, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml, const float* __restrict__ part_o) {
+    constexpr int Q = D / 4, R = 256 / Q;                    // threads of one share, shares at once
+    __shared__ float weight[256], sums[256];
+    __shared__ f4 acc[256];
+    const int64_t row = blockIdx.x;
+    const int parts = min(used[row], splits);
+    if (parts <= 1) return;
+    const int t = threadIdx.x;
+    const float2 ml = t < parts ? part_ml[row * splits + t] : float2{-INFINITY, 0.f};
+    weight[t] = ml.x;
+    __syncthreads();
+    float top = -INFINITY;
+    for (int i = 0; i < parts; ++i) top = fmaxf(top, weight[i]);
+    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+    __syncthreads();
+    weight[t] = f;
+    sums[t] = f * ml.y;
+    __syncthreads();
+    float sum = 0.f;
+    for (int i = 0; i < parts; ++i) sum += sums[i];
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = t / Q; i < parts; i += R) v += weight[i] * *reinterpret_cast<const f4*>(part_o + (row * splits + i) * D + t % Q * 4);
+    acc[t] = v;
+    __syncthreads();
+    if (t >= Q) return;
+    for (int i = 1; i < R; ++i) v += acc[i * Q + t];
+    kv4_finish<D>(a, row, 4 * t, top, sum, v[0], v[1]);
+    kv4_finish<D>(a, row, 4 * t + 2, top, sum, v[2], v[3]);
+}
+
 static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_attention_args* a, const w4a16_device_limits* lim) {
     if (const char* m = kv4_check(c)) return m;
     if (!a || !lim) return "null pointer";
     if (a->tokens < 0 || a->batch < 0 || a->table_width < 0 || a->heads < 1 || a->heads > 4096 || a->tokens >= (int64_t)1 << 31 ||
-        a->batch >= (int64_t)1 << 20 || a->table_width * c->page_size >= (int64_t)1 << 31 || a->max_q < 1 || a->window < 0 ||
+        a->batch >= 65536 || a->table_width * c->page_size >= (int64_t)1 << 27 || a->max_q < 1 || a->window < 0 ||
         a->tokens * a->heads >= (int64_t)1 << 31 || a->batch * a->heads >= (int64_t)1 << 31)
         return "dimensions out of range";
     if (a->heads % c->kv_heads != 0) return "the query heads must be a multiple of the KV heads";
@@ -112,6 +568,32 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
     return nullptr;
 }
 
+// How a call runs: rows of one pass of the token kernel (4 nt; 0: the other kernel), shares of the keys of one row, and
+// the workspace: per row (query, query head) the number of shares, then (largest score, sum) and sums of each share.
+struct AttnPlan {
+    int nt, splits;
+    int64_t ml_at, o_at, bytes;
+};
+
+static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attention_args& a) {
+    AttnPlan p{};
+    const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep;
+    p.splits = 1;
+    if (rows > 16) return p;
+    p.nt = rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
+    int64_t tiles = (a.table_width * c.page_size + 63) / 64;
+    if (a.window > 0) tiles = std::min(tiles, (a.window + a.max_q) / 64 + 2);
+    const int64_t wanted = 2048 / (a.batch * c.kv_heads);
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + 3) / 4, 256}));
+    if (p.splits > 1) {
+        const int64_t all = a.tokens * a.heads;
+        p.ml_at = (all * 4 + 15) / 16 * 16;
+        p.o_at = (p.ml_at + all * p.splits * 8 + 15) / 16 * 16;
+        p.bytes = p.o_at + all * p.splits * c.head_dim * 4;
+    }
+    return p;
+}
+
 }  // namespace w4a16
 
 using namespace w4a16;
@@ -119,7 +601,7 @@ using namespace w4a16;
 extern "C" int64_t w4a16_kv4_attention_workspace(const w4a16_kv4_cache* cache, const w4a16_kv4_attention_args* args,
                                                  const w4a16_device_limits* lim) {
     if (const char* m = check_attention(cache, args, lim)) return kv4_fail(-1, "kv4_attention", m);
-    return 0;
+    return args->tokens == 0 || args->batch == 0 ? 0 : plan_attention(*cache, *args).bytes;
 }
 
 extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4_attention_args* args, const w4a16_device_limits* lim,
@@ -148,10 +630,30 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
     a.scale2 = args->scale * 1.44269504088896341f;
     a.bf16 = args->bf16 != 0;
     a.causal = args->causal != 0;
-    const dim3 grid((unsigned)(args->batch * args->heads), (unsigned)(args->max_q < 65535 ? args->max_q : 65535));
-    hipStream_t st = (hipStream_t)stream;
+    a.q_wide = reinterpret_cast<uintptr_t>(args->q) % 16 == 0 && args->q_token_stride % 8 == 0 && args->q_head_stride % 8 == 0;
+    const AttnPlan plan = plan_attention(*cache, *args);
+    const hipStream_t st = (hipStream_t)stream;
+    char* const ws = (char*)workspace;
+    int* const used = plan.splits > 1 ? (int*)ws : nullptr;
+    float2* const ml = (float2*)(ws + plan.ml_at);
+    float* const po = (float*)(ws + plan.o_at);
     kv4_sizes(cache, [&](auto d, auto g) {
-        hipLaunchKernelGGL((kv4_attention_kernel<d.value, g.value>), grid, dim3(64), 0, st, a);
+        if (plan.nt) {
+            const uint32_t magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)(cache->page_size / 16) + 1);
+            const dim3 grid((unsigned)(cache->kv_heads * plan.splits), (unsigned)args->batch);
+            auto launch = [&](auto nt) {
+                hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4>), grid, dim3(256), 0, st, a, plan.splits, magic, used, ml, po);
+            };
+            if (plan.nt == 1) launch(std::integral_constant<int, 1>{});
+            else if (plan.nt == 2) launch(std::integral_constant<int, 2>{});
+            else launch(std::integral_constant<int, 4>{});
+            if (plan.splits > 1)
+                hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits,
+                                   used, ml, po);
+        } else {
+            const dim3 grid((unsigned)(args->batch * args->heads), (unsigned)(args->max_q < 65535 ? args->max_q : 65535));
+            hipLaunchKernelGGL((kv4_attention_kernel<d.value, g.value>), grid, dim3(64), 0, st, a);
+        }
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_attention", hipGetErrorString(e));
     return W4A16_OK;
