@@ -18,92 +18,6 @@ __device__ __forceinline__ void kv4_finish(const Kv4Attn& a, int64_t row, int d,
     if (d == 0 && a.lse) a.lse[row] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.69314718055994531f;
 }
 
-// One wave per (query, query head).  Keys go by in tiles of 64: lane t takes the score of key t, the tile's
-// probabilities pass through LDS, and lane d adds up values d and d + D/2.
-template <int D, int G>
-__global__ void __launch_bounds__(64)
-kv4_attention_kernel(Kv4Attn a) {
-    __shared__ float qs[D], ps[64];
-    __shared__ int pages[64];
-    constexpr int NG = D / G, HALF = D / 2;
-    const int lane = threadIdx.x;
-    const int b = blockIdx.x / a.heads, head = blockIdx.x % a.heads, h = head / a.rep;
-    const Kv4Seq s = kv4_seq(a, b);
-    for (int i = blockIdx.y; i < s.count; i += gridDim.y) {
-        const int64_t row = s.first + i;
-        const int pos = s.len - s.count + i;
-        const int end = a.causal ? min(pos + 1, s.len) : s.len;
-        const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-        __syncthreads();
-        for (int d = lane; d < D; d += 64) qs[d] = load16(a.q[row * a.q_token + head * a.q_head + d], a.bf16) * a.scale2;
-        __syncthreads();
-        float top = -INFINITY, total = 0.f, o0 = 0.f, o1 = 0.f;
-        for (int t0 = begin & ~15; t0 < end; t0 += 64) {
-            const int t = t0 + lane;
-            int page = t < end && t >= begin ? a.table[b * a.table_stride + t / a.c.P] : -1;
-            if (page >= a.c.pages) page = -1;
-            float x = -INFINITY;
-            if (page >= 0) {
-                const uint8_t* kv = a.c.head(page, h);
-                const int at = t % a.c.P;
-                x = 0.f;
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const float sc = half_bits(*(const uint16_t*)(kv + kv4_side<D, G>(a.c.P, kKeyScale, g, at)));
-                    const float ze = half_bits(*(const uint16_t*)(kv + kv4_side<D, G>(a.c.P, kKeyZero, g, at)));
-                    float dot = 0.f;
-                    for (int j = 0; j < G; ++j) {
-                        const int d = g * G + j;
-                        const uint32_t byte = kv[kv4_key_row<D>(at) + d % HALF];
-                        dot += qs[d] * ((float)((d < HALF ? byte : byte >> 4) & 15u) - ze);
-                    }
-                    x += dot * sc;
-                }
-            }
-            float m = x;
-            for (int w = 1; w < 64; w *= 2) m = fmaxf(m, __shfl_xor(m, w, 64));
-            const bool nan = __any(x != x);
-            const float next = nan ? NAN : fmaxf(top, m);
-            const float safe = next == -INFINITY ? 0.f : next;
-            const float p = page >= 0 ? exp2f(x - safe) : 0.f;
-            float sum = p;
-            for (int w = 1; w < 64; w *= 2) sum += __shfl_xor(sum, w, 64);
-            const float keep = exp2f(top - safe);
-            total = total * keep + sum;
-            o0 *= keep;
-            o1 *= keep;
-            top = next;
-            __syncthreads();
-            ps[lane] = p;
-            pages[lane] = page;
-            __syncthreads();
-            if (lane < HALF) {
-                for (int r = 0; r < 64; ++r) {
-                    const int pg = pages[r];
-                    if (pg < 0) continue;
-                    const uint8_t* kv = a.c.head(pg, h);
-                    const int at = (t0 + r) % a.c.P;
-                    const uint32_t byte = kv[kv4_value_tile<D>(a.c.P, at) + lane * 16 + kv4_place(at & 15)];
-                    const int g0 = lane / G, g1 = (lane + HALF) / G;
-                    const float s0 = half_bits(*(const uint16_t*)(kv + kv4_side<D, G>(a.c.P, kValueScale, g0, at)));
-                    const float z0 = half_bits(*(const uint16_t*)(kv + kv4_side<D, G>(a.c.P, kValueZero, g0, at)));
-                    const float s1 = half_bits(*(const uint16_t*)(kv + kv4_side<D, G>(a.c.P, kValueScale, g1, at)));
-                    const float z1 = half_bits(*(const uint16_t*)(kv + kv4_side<D, G>(a.c.P, kValueZero, g1, at)));
-                    o0 += ps[r] * (((float)(byte & 15u) - z0) * s0);
-                    o1 += ps[r] * (((float)(byte >> 4) - z1) * s1);
-                }
-            }
-        }
-        const float inv = total == 0.f ? 0.f : 1.f / total;   // a row that sees nothing: zeros; NaN stays NaN
-        uint16_t* dst = a.out + (row * a.heads + head) * D;
-        if (lane < HALF) {
-            dst[lane] = store16(o0 * inv, a.bf16);
-            dst[lane + HALF] = store16(o1 * inv, a.bf16);
-        }
-        if (a.lse && lane == 0) a.lse[row * a.heads + head] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
-    }
-}
-
 // ------------------------------------------------------------------------------------------------
 // Few rows (single tokens, drafts): kv4_token_kernel
 
@@ -548,6 +462,377 @@ kv4_join_kernel(Kv4Attn a, int splits, const int* __restrict__ used, const float
     kv4_finish<D>(a, row, 4 * t + 2, top, sum, v[2], v[3]);
 }
 
+// ------------------------------------------------------------------------------------------------
+// Many rows (chunks, prompts): kv4_prompt_kernel
+
+__device__ __forceinline__ h2 as_h2(uint32_t v) { return __builtin_bit_cast(h2, v); }
+__device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uint32_t, v); }
+
+// The eight codes of a dword less their zeros, in fp16: c | 0x6400 in bits 4..7 of a half is 1024 + 16 c, which one
+// FMA takes to c - z exactly (less = -64 - z).  lo0 and lo1 hold the lower codes of bytes 0, 2 and 1, 3, hi0 and hi1
+// the upper ones.
+__device__ __forceinline__ void expand(uint32_t w, h2 less_lo0, h2 less_lo1, h2 less_hi0, h2 less_hi1, uint32_t& lo0, uint32_t& lo1,
+                                       uint32_t& hi0, uint32_t& hi1) {
+    constexpr uint32_t mask = 0x00F000F0u, magic = 0x64006400u;
+    const h2 f = {(_Float16)0.0625f, (_Float16)0.0625f};
+    lo0 = as_u32(__builtin_elementwise_fma(as_h2(((w << 4) & mask) | magic), f, less_lo0));
+    hi0 = as_u32(__builtin_elementwise_fma(as_h2((w & mask) | magic), f, less_hi0));
+    lo1 = as_u32(__builtin_elementwise_fma(as_h2(((w >> 4) & mask) | magic), f, less_lo1));
+    hi1 = as_u32(__builtin_elementwise_fma(as_h2(((w >> 8) & mask) | magic), f, less_hi1));
+}
+// -64 - z for two zeros; a NaN or anything past the format's range (which only unwritten places hold) becomes finite.
+__device__ __forceinline__ h2 less_of(uint32_t z) {
+    const h2 most = {(_Float16)97.f, (_Float16)97.f}, base = {(_Float16)-64.f, (_Float16)-64.f};
+    return base - __builtin_elementwise_min(__builtin_elementwise_max(as_h2(z), -most), most);
+}
+__device__ __forceinline__ float other_half(float v) {       // the value of lane ^ 32
+    return __shfl_xor(v, 32, 64);
+}
+
+// One workgroup takes 32 WAVES rows (query, query head) of one KV head and a share of their keys, in tiles of 64 that
+// all waves share through LDS as c - z in fp16, which is exact; a wave has 32 rows.  S^T = K Q^T, so a lane has one row's
+// scores (v_mfma_f32_32x32x16_f16: column lane % 32) and keeps that row's statistics to itself; its probabilities times
+// the values' scales are already where O^T = V^T P^T takes them from.  Scales are applied to the scores, so that only
+// the query (exact in fp16, a bf16 row times a power of two) and p s, rounded to fp16, are operands.
+// A row's reference `top` lies 2^7 under its largest score times the largest value scale seen: p s < 2^15 until that has
+// grown by 2^8, and only then are the sums scaled again.
+template <int D, int G, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
+kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
+                  float* __restrict__ part_o) {
+    constexpr int NG = D / G, BM = 32 * WAVES;
+    constexpr int kKeyRow = D * 2 + 16, kValRow = 144;       // LDS rows: a token's values; 64 tokens of one value
+    constexpr int kVal = 64 * kKeyRow, kSk = kVal + D * kValRow, kSv = kSk + NG * 256, kEv = kSv + NG * 256, kBuf = kEv + 32;
+    constexpr int kPieces = 64 * D / 32;                     // 16-byte pieces of a tile's keys, and of its values
+    static_assert(WAVES == 4, "a thread has one piece of keys and one of values, or waves 0 and 1 keys and 2 and 3 values");
+    constexpr int PER = D / 64;
+    __shared__ __align__(16) uint8_t lds[2 * kBuf];
+    const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = blockIdx.x, split = blockIdx.y % splits, b = blockIdx.z;
+    const Kv4Seq s = kv4_seq(a, b);
+    const int rows = s.count * a.rep, base = s.len - s.count, groups = a.c.P >> 4;
+    const int* const table = a.table + b * a.table_stride;
+    const int all = (rows + BM - 1) / BM;
+
+    // the last rows first: with causal attention they have the most keys
+    for (int index = blockIdx.y / splits; index < all; index += row_tiles) {
+        const int row0 = (all - 1 - index) * BM;
+        const int first = row0 / a.rep, last = (min(row0 + BM, rows) - 1) / a.rep;
+        const int kmax = a.causal ? max(0, min(base + last + 1, s.len)) : s.len;
+        const int kmin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
+        const int tile0 = kmin >> 6, tiles = a.c.pages > 0 ? max(0, ((kmax + 63) >> 6) - tile0) : 0;
+        const int per = max(4, (tiles + splits - 1) / splits), parts = max(1, (tiles + per - 1) / per);
+        if (split >= parts) continue;
+        const int stop = tile0 + min(tiles, (split + 1) * per);
+
+        // this wave's rows: the keys that any and all of them see, and this lane's row
+        const int wr0 = row0 + 32 * wave, wr1 = min(wr0 + 32, rows) - 1;
+        const int wfirst = wr0 / a.rep, wlast = wr1 / a.rep;
+        const int any_end = wr0 >= rows ? 0 : a.causal ? min(base + wlast + 1, s.len) : s.len;
+        const int any_begin = a.window > 0 ? max(0, base + wfirst - a.window + 1) : 0;
+        const int sure_end = a.causal ? min(base + wfirst + 1, s.len) : s.len;
+        const int sure_begin = a.window > 0 ? max(0, base + wlast - a.window + 1) : 0;
+        const int row = wr0 + col, query = row / a.rep, head = h * a.rep + row % a.rep, pos = base + query;
+        const int end = row < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
+        const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+
+        // The lane's query in fp16, values in the order of the keys' LDS rows: within four, 0 2 1 3
+        h8 q[D / 16];
+        float rowf = 1.f;
+        {
+            u4 w[D / 16];
+            uint32_t big = 0;
+            const int safe = min(row, rows - 1);             // rows past the last compute it again, unused
+            const uint16_t* src = a.q + (int64_t)(s.first + safe / a.rep) * a.q_token + (int64_t)(h * a.rep + safe % a.rep) * a.q_head + 8 * half;
+            if (a.q_wide) {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i) w[i] = *reinterpret_cast<const u4*>(src + 16 * i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[i][j] = (uint32_t)src[16 * i + 2 * j] | ((uint32_t)src[16 * i + 2 * j + 1] << 16);
+            }
+            auto value = [&](int i, int j) {
+                const uint32_t v = w[i][j >> 1];
+                return load16((j & 1 ? v >> 16 : v) & 0xFFFF, a.bf16);
+            };
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) big = max(big, __builtin_bit_cast(uint32_t, value(i, j)) & 0x7FFFFFFFu);
+            big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+            int e = 0;
+            if (a.bf16) {                                    // the row's largest to 2^7 .. 2^8
+                e = big < 0x7F800000u ? min(max(__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, big)) - 8, -110), 110) : 0;
+                rowf = ldexpf(1.f, e);
+            }
+            if (big >= 0x7F800000u) rowf = NAN;
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int from = (j & 4) | ((j & 1) << 1) | ((j >> 1) & 1);
+                    q[i][j] = (_Float16)ldexpf(value(i, from), -e);
+                }
+            }
+        }
+
+        float top = -INFINITY, total = 0.f;
+        f32x16 o[D / 32];
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
+
+        // Each thread's pieces of a tile: 16 bytes of a token's keys, and of 16 tokens' values
+        struct Piece {
+            u4 w, z[2][NG];
+            uint16_t zk[NG], s[NG];
+            bool there;
+        };
+        auto keys = [&](int i) { return D == 128 ? i == 0 : wave < 2; };
+        const int p = D == 128 ? tid : tid & 127, mine = p / (kPieces / 4);
+        auto entry = [&](int tile) {
+            const int group = tile * 4 + mine;
+            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
+            return group * 16 < kmax ? table[at] : -1;
+        };
+        auto load = [&](int tile, int i, int page, Piece& x) {
+            const int group = tile * 4 + mine;
+            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
+            const int place = (group - at * groups) * 16;
+            x.there = (uint32_t)page < (uint32_t)a.c.pages;
+            const uint8_t* kv = a.c.head(x.there ? page : 0, h);
+            if (keys(i)) {
+                const int token = place + p / (D / 32) % 16;
+                x.w = *reinterpret_cast<const u4*>(kv + kv4_key_row<D>(token) + p % (D / 32) * 16);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    x.zk[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, kKeyZero, g, token));
+                    x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, kKeyScale, g, token));
+                }
+            } else {
+                const int j = p % (D / 2);
+                x.w = *reinterpret_cast<const u4*>(kv + kv4_value_tile<D>(a.c.P, place) + j * 16);
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    const u4* z = reinterpret_cast<const u4*>(kv + kv4_side<D, G>(a.c.P, kValueZero, g, place));
+                    x.z[0][g] = z[0];
+                    x.z[1][g] = z[1];
+                    x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, kValueScale, g, place + (j & 15)));
+                }
+            }
+        };
+        auto put = [&](int tile, int i, const Piece& x, uint8_t* buf) {
+            const int group = mine;
+            if (keys(i)) {
+                const int token = p / (D / 32), c = p % (D / 32);
+                const h2 lo = less_of(x.zk[0] * 0x10001u), hi = less_of(x.zk[NG - 1] * 0x10001u);
+                u4 l0, l1, h0, h1;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t a0, a1, b0, b1;
+                    expand(x.w[j], lo, lo, hi, hi, a0, a1, b0, b1);
+                    u4& l = j < 2 ? l0 : l1;
+                    u4& u = j < 2 ? h0 : h1;
+                    l[2 * (j & 1)] = a0;
+                    l[2 * (j & 1) + 1] = a1;
+                    u[2 * (j & 1)] = b0;
+                    u[2 * (j & 1) + 1] = b1;
+                }
+                uint8_t* at = buf + token * kKeyRow + c * 32;
+                *reinterpret_cast<u4*>(at) = l0;
+                *reinterpret_cast<u4*>(at + 16) = l1;
+                *reinterpret_cast<u4*>(at + D) = h0;
+                *reinterpret_cast<u4*>(at + D + 16) = h1;
+                if (c == 0) {
+                    const bool live = x.there && tile * 64 + token < kmax;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g)
+                        *reinterpret_cast<float*>(buf + kSk + g * 256 + token * 4) = live ? half_bits(x.s[g]) * a.scale2 : 0.f;
+                }
+            } else {
+                const int j = p % (D / 2);
+                u4 l[2], u[2];                               // tokens 0-3 and 8-11, 4-7 and 12-15: a lane half's operand
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint32_t z0 = x.z[i >> 1][0][2 * (i & 1)], z1 = x.z[i >> 1][0][2 * (i & 1) + 1];
+                    const uint32_t y0 = x.z[i >> 1][NG - 1][2 * (i & 1)], y1 = x.z[i >> 1][NG - 1][2 * (i & 1) + 1];
+                    uint32_t a0, a1, b0, b1;
+                    expand(x.w[i], less_of(z0), less_of(z1), less_of(y0), less_of(y1), a0, a1, b0, b1);
+                    l[i & 1][i & 2] = a0;
+                    l[i & 1][(i & 2) + 1] = a1;
+                    u[i & 1][i & 2] = b0;
+                    u[i & 1][(i & 2) + 1] = b1;
+                }
+                uint8_t* at = buf + kVal + j * kValRow + group * 32;
+                *reinterpret_cast<u4*>(at) = l[0];
+                *reinterpret_cast<u4*>(at + 16) = l[1];
+                *reinterpret_cast<u4*>(at + D / 2 * kValRow) = u[0];
+                *reinterpret_cast<u4*>(at + D / 2 * kValRow + 16) = u[1];
+                if (j < 16) {
+                    const bool live = x.there && tile * 64 + group * 16 + j < kmax;
+                    int most = 0;
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) {
+                        *reinterpret_cast<float*>(buf + kSv + g * 256 + (group * 16 + j) * 4) = live ? half_bits(x.s[g]) : 0.f;
+                        most = max(most, live ? min((int)x.s[g], 0x7BFF) : 0);
+                    }
+                    W4A16_OVER_ROW(most, max);
+                    if (j == 0) {
+                        *reinterpret_cast<int*>(buf + kEv + group * 4) = (most >> 10) - 14;     // the scales are under 2^that
+                        *reinterpret_cast<int*>(buf + kEv + 16 + group * 4) = x.there;
+                    }
+                }
+            }
+        };
+
+        // Turn t puts tile t + 1 into one LDS buffer, sends for tile t + 2 and computes tile t from the other buffer.
+        Piece x[PER];
+        const int start = tile0 + split * per;
+        int page = start < stop ? entry(start) : -1;
+        if (start < stop) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) load(start, i, page, x[i]);
+        }
+        if (start + 1 < stop) page = entry(start + 1);
+        uint8_t *buf = lds, *other = lds + kBuf;
+        for (int tile = start - 1; tile < stop; ++tile) {
+            if (tile >= start) __syncthreads();              // this tile is in LDS, and nobody reads the other buffer
+            if (tile + 1 < stop) {
+#pragma unroll
+                for (int i = 0; i < PER; ++i) {
+                    put(tile + 1, i, x[i], other);
+                    if (tile + 2 < stop) load(tile + 2, i, page, x[i]);
+                }
+                if (tile + 3 < stop) page = entry(tile + 3);
+            }
+            uint8_t* const now = buf;
+            buf = other;
+            other = now;
+            if (tile < start || tile * 64 >= any_end || tile * 64 + 64 <= any_begin) continue;
+
+            f32x16 y[2];
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int g = 0; g < NG; ++g) {
+                    f32x16 acc;
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
+#pragma unroll
+                    for (int i = g * G / 16; i < (g + 1) * G / 16; ++i) {
+                        const h8 k = *reinterpret_cast<const h8*>(now + (32 * tb + col) * kKeyRow + i * 32 + half * 16);
+                        acc = mfma32x32x16(k, q[i], acc);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const f4 sk = *reinterpret_cast<const f4*>(now + kSk + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            y[tb][4 * j + i] = g == 0 ? acc[4 * j + i] * sk[i] : fmaf(acc[4 * j + i], sk[i], y[tb][4 * j + i]);
+                    }
+                    if constexpr (NG == 2) __builtin_amdgcn_sched_barrier(0);    // one set of sums at a time: registers
+                }
+            const i4v evs = *reinterpret_cast<const i4v*>(now + kEv), flags = *reinterpret_cast<const i4v*>(now + kEv + 16);
+            const int ev = max(max(evs[0], evs[1]), max(evs[2], evs[3]));
+            const bool there = __builtin_amdgcn_readfirstlane(flags[0] & flags[1] & flags[2] & flags[3]) != 0;
+            const bool whole = there && tile * 64 + 64 <= sure_end && tile * 64 >= sure_begin;
+            if (!whole) {
+#pragma unroll
+                for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const int at = tile * 64 + 4 * half + 32 * tb + 8 * (j >> 2) + (j & 3);
+                        const bool see = (int)(at < end) & (int)(at >= begin) & flags[2 * tb + (j >> 3)];
+                        y[tb][j] = see ? y[tb][j] : -INFINITY;
+                    }
+            }
+            float most = y[0][0];
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) most = fmaxf(most, y[tb][j]);
+            most = fmaxf(most, other_half(most)) * rowf;
+            const float need = most + (float)(ev - 7);
+            if (__any(need > top + 8.f)) {                   // also where a row sees its first key: top is -inf
+                const float next = fmaxf(top, need);
+                const float keep = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
+                top = next;
+                total *= keep;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) o[i][j] *= keep;
+            }
+            const float safe = top == -INFINITY ? 0.f : -top;
+#pragma unroll
+            for (int tb = 0; tb < 2; ++tb) {
+                h8 ps[NG][2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f4 sv[NG];
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) sv[g] = *reinterpret_cast<const f4*>(now + kSv + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(y[tb][4 * j + i], rowf, safe));
+                        total += e;
+#pragma unroll
+                        for (int g = 0; g < NG; ++g) {
+                            float v = e * sv[g][i];
+                            if (!whole && e == 0.f) v = 0.f;         // a token that another row sees may hold NaN
+                            ps[g][j >> 1][4 * (j & 1) + i] = (_Float16)v;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const h8 v = *reinterpret_cast<const h8*>(now + kVal + (32 * i + col) * kValRow + (2 * tb + k) * 32 + half * 16);
+                        o[i] = mfma32x32x16(v, ps[NG == 2 ? i / (D / 64) : 0][k], o[i]);
+                    }
+            }
+        }
+
+        total += other_half(total);
+        if (row < rows) {
+            const int64_t at = (int64_t)(s.first + query) * a.heads + head;
+            if (parts == 1) {
+                const float inv = total == 0.f ? 0.f : 1.f / total;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t w0 = (uint32_t)store16(o[i][4 * j] * inv, a.bf16) | ((uint32_t)store16(o[i][4 * j + 1] * inv, a.bf16) << 16);
+                        const uint32_t w1 = (uint32_t)store16(o[i][4 * j + 2] * inv, a.bf16) | ((uint32_t)store16(o[i][4 * j + 3] * inv, a.bf16) << 16);
+                        *reinterpret_cast<u2*>(a.out + at * D + 32 * i + 8 * j + 4 * half) = u2{w0, w1};
+                    }
+                if (half == 0) {
+                    if (a.lse) a.lse[at] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
+                    if (used) used[at] = 1;
+                }
+            } else {
+                const int64_t share = at * splits + split;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        *reinterpret_cast<f4*>(part_o + share * D + 32 * i + 8 * j + 4 * half) =
+                            f4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
+                if (half == 0) {
+                    part_ml[share] = float2{top, total};
+                    if (split == 0) used[at] = parts;
+                }
+            }
+        }
+        __syncthreads();                                     // before the next rows' first tile goes into LDS
+    }
+}
+
 static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_attention_args* a, const w4a16_device_limits* lim) {
     if (const char* m = kv4_check(c)) return m;
     if (!a || !lim) return "null pointer";
@@ -568,10 +853,11 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
     return nullptr;
 }
 
-// How a call runs: rows of one pass of the token kernel (4 nt; 0: the other kernel), shares of the keys of one row, and
+// How a call runs: rows of one pass of the token kernel (4 nt; 0: the prompt kernel, row_tiles workgroups), shares of the keys of one row, and
 // the workspace: per row (query, query head) the number of shares, then (largest score, sum) and sums of each share.
+constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
 struct AttnPlan {
-    int nt, splits;
+    int nt, splits, row_tiles;
     int64_t ml_at, o_at, bytes;
 };
 
@@ -579,11 +865,16 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
     AttnPlan p{};
     const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep;
     p.splits = 1;
-    if (rows > 16) return p;
-    p.nt = rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
     int64_t tiles = (a.table_width * c.page_size + 63) / 64;
     if (a.window > 0) tiles = std::min(tiles, (a.window + a.max_q) / 64 + 2);
-    const int64_t wanted = 2048 / (a.batch * c.kv_heads);
+    int64_t wanted;
+    if (rows <= 16) {
+        p.nt = rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
+        wanted = 2048 / (a.batch * c.kv_heads);
+    } else {
+        p.row_tiles = (int)std::min<int64_t>((rows + kPromptRows - 1) / kPromptRows, 65535);
+        wanted = 512 / (a.batch * c.kv_heads * p.row_tiles);
+    }
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + 3) / 4, 256}));
     if (p.splits > 1) {
         const int64_t all = a.tokens * a.heads;
@@ -638,8 +929,8 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
     float2* const ml = (float2*)(ws + plan.ml_at);
     float* const po = (float*)(ws + plan.o_at);
     kv4_sizes(cache, [&](auto d, auto g) {
+        const uint32_t magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)(cache->page_size / 16) + 1);
         if (plan.nt) {
-            const uint32_t magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)(cache->page_size / 16) + 1);
             const dim3 grid((unsigned)(cache->kv_heads * plan.splits), (unsigned)args->batch);
             auto launch = [&](auto nt) {
                 hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4>), grid, dim3(256), 0, st, a, plan.splits, magic, used, ml, po);
@@ -647,13 +938,14 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
             if (plan.nt == 1) launch(std::integral_constant<int, 1>{});
             else if (plan.nt == 2) launch(std::integral_constant<int, 2>{});
             else launch(std::integral_constant<int, 4>{});
-            if (plan.splits > 1)
-                hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits,
-                                   used, ml, po);
         } else {
-            const dim3 grid((unsigned)(args->batch * args->heads), (unsigned)(args->max_q < 65535 ? args->max_q : 65535));
-            hipLaunchKernelGGL((kv4_attention_kernel<d.value, g.value>), grid, dim3(64), 0, st, a);
+            const dim3 grid((unsigned)cache->kv_heads, (unsigned)(plan.row_tiles * plan.splits), (unsigned)args->batch);
+            hipLaunchKernelGGL((kv4_prompt_kernel<d.value, g.value, kPromptWaves>), grid, dim3(64 * kPromptWaves), 0, st, a, plan.row_tiles,
+                               plan.splits, magic, used, ml, po);
         }
+        if (plan.splits > 1)
+            hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits, used,
+                               ml, po);
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_attention", hipGetErrorString(e));
     return W4A16_OK;
