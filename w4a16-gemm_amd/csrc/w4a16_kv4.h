@@ -14,11 +14,13 @@ namespace w4a16 {
 // A cache as the kernels take it.
 struct Kv4 {
     uint8_t* data;
-    int64_t head_bytes;                      // bytes of one (page, KV head)
+    uint32_t head_bytes, page_bytes;         // bytes of one (page, KV head), and of one page (at most 576 MiB)
     int pages, P, H;
 
     __host__ __device__ int64_t slots() const { return (int64_t)pages * P; }
-    __device__ uint8_t* head(int page, int h) const { return data + ((int64_t)page * H + h) * head_bytes; }
+    __device__ uint8_t* head(int page, int h) const {
+        return data + (uint64_t)(uint32_t)h * head_bytes + (uint64_t)(uint32_t)page * page_bytes;
+    }
 };
 
 enum { kKeyScale = 0, kKeyZero = 1, kValueScale = 2, kValueZero = 3 };
@@ -38,6 +40,18 @@ __device__ __forceinline__ int kv4_side(int P, int which, int group, int t) {
 
 __device__ __forceinline__ float half_bits(uint16_t b) { return (float)__builtin_bit_cast(_Float16, b); }
 __device__ __forceinline__ uint16_t to_half_bits(float v) { return __builtin_bit_cast(uint16_t, (_Float16)v); }
+
+// The value of another lane of the row of 16: the neighbour, the pair over, the four and the eight mirrored.
+template <int CTRL>
+__device__ __forceinline__ int dpp(int v) {
+    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(int, v)));
+}
+constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+constexpr int kShiftDown = 0x100;            // + n: lane i gets lane i + n's, 0 past the row's end
 
 // 16-bit inputs and outputs, fp16 or bf16.
 __device__ __forceinline__ float load16(uint16_t b, bool bf16) {

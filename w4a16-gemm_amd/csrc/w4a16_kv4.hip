@@ -6,91 +6,228 @@
 
 namespace w4a16 {
 
-// One wave per (token, KV head) of K (blockIdx.y even) or V.  Lane j holds values j and j + D/2, the two
-// codes of byte j.  Every operation is an IEEE fp32 operation, so the bytes are the format's definition.
-template <int D, int G>
-__global__ void __launch_bounds__(256)
-kv4_write_kernel(Kv4 c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int bf16, int tokens, int64_t k_token,
-                 int64_t k_head, int64_t v_token, int64_t v_head, const int64_t* __restrict__ slots) {
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+// Tokens go by in windows of W, one KV head at a time; D / 8 lanes of eight values share a token.  The value codes of 16
+// tokens lie interleaved in 16-byte pieces, so where a window's slots hold a whole aligned run of 16 (a prompt), the
+// pieces pass through LDS and global memory sees 16-byte accesses; other tokens (single ones, the ends of a run)
+// take their bytes one at a time.
+
+// The page of a slot in the cache, and the place in it: both fit 32 bits once the 16-token groups are counted.
+__device__ __forceinline__ int kv4_page(const Kv4& c, int64_t slot, int& at) {
+    const uint32_t group = (uint32_t)(slot >> 4), per = (uint32_t)c.P >> 4, page = group / per;
+    at = (int)(((group - page * per) << 4) | ((uint32_t)slot & 15u));
+    return (int)page;
+}
+
+// Bit i of the result: tokens i .. i + 15 of the window are the 16 slots of one aligned group, in order.
+template <int W>
+__device__ __forceinline__ uint64_t kv4_runs(const int64_t* slots, int tokens, int64_t most) {
     const int lane = threadIdx.x & 63;
-    const int64_t token = unit / c.H;
-    const int h = (int)(unit % c.H);
-    if (token >= tokens) return;
-    const int64_t slot = slots[token];
-    if (slot < 0 || slot >= c.slots()) return;
-    const bool value = blockIdx.y != 0;
-    const uint16_t* src = value ? v + token * v_token + h * v_head : k + token * k_token + h * k_head;
-    const bool live = lane < D / 2;
-    const float x0 = live ? load16(src[lane], bf16) : 0.f, x1 = live ? load16(src[lane + D / 2], bf16) : 0.f;
-    float x[2] = {fminf(fmaxf(x0, -65504.f), 65504.f), fminf(fmaxf(x1, -65504.f), 65504.f)};
-    const bool nan[2] = {x0 != x0, x1 != x1};
-    constexpr int NG = D / G;
-    float lo[NG], hi[NG], s[NG], z[NG];
-    bool bad[NG];
-#pragma unroll
-    for (int g = 0; g < NG; ++g) {
-        lo[g] = NG == 2 ? x[g] : fminf(x[0], x[1]);
-        hi[g] = NG == 2 ? x[g] : fmaxf(x[0], x[1]);
-        if (!live) lo[g] = INFINITY, hi[g] = -INFINITY;
-#pragma unroll
-        for (int m = 1; m < 64; m *= 2) {
-            lo[g] = fminf(lo[g], __shfl_xor(lo[g], m, 64));
-            hi[g] = fmaxf(hi[g], __shfl_xor(hi[g], m, 64));
-        }
-        bad[g] = __any(NG == 2 ? nan[g] : nan[0] || nan[1]);
-        const float step = fmaxf(fmaxf((hi[g] - lo[g]) / 15.f, fmaxf(fabsf(lo[g]), fabsf(hi[g])) / 96.f), 0x1p-14f);
-        s[g] = half_bits(to_half_bits(step));
-        z[g] = rintf(-lo[g] / s[g] * 8.f) / 8.f;
-    }
-    uint32_t q[2];
+    const bool in = lane < W && lane < tokens;
+    const int64_t s = in ? slots[lane] : -1;
+    const int next_lo = __shfl_down((int)(uint32_t)s, 1, 64), next_hi = __shfl_down((int)(s >> 32), 1, 64);
+    const int64_t next = ((int64_t)next_hi << 32) | (uint32_t)next_lo;
+    const uint64_t follows = __ballot(in && lane < 63 && next == s + 1);
+    return __ballot(in && s >= 0 && s < most && s % 16 == 0 && ((follows >> lane) & 0x7FFF) == 0x7FFF);
+}
+// The run that holds token t of the window: its number, and where it starts; -1 if none does.
+__device__ __forceinline__ int kv4_run_of(uint64_t runs, int t, int& start) {
+    const uint64_t upto = runs & ((uint64_t)2 << t) - 1;
+    start = 63 - __clzll((long long)upto);
+    return upto && t - start < 16 ? __popcll(upto) - 1 : -1;
+}
+__device__ __forceinline__ int kv4_run_start(uint64_t runs, int which) {
+    for (int i = 0; i < which; ++i) runs &= runs - 1;
+    return __ffsll((unsigned long long)runs) - 1;
+}
+
+// Over the 8 or 16 lanes of a token's group of values.
+template <int LANES, typename T, class F>
+__device__ __forceinline__ T over_lanes(T v, F f) {
+    v = f(v, dpp<kXor1>(v));
+    v = f(v, dpp<kXor2>(v));
+    v = f(v, dpp<kHalfMirror>(v));
+    if constexpr (LANES == 16) v = f(v, dpp<kMirror>(v));
+    return v;
+}
+
+// Every operation is an IEEE fp32 operation or agrees with one, so the bytes are the format's definition.  The codes'
+// quotient x / s is taken as x rcp(s) first: with |x / s| < 113 the two differ by less than 2^-16, so only a value
+// whose x rcp(s) + z is within 2^-15 of a half-integer needs the division.
+template <int D, int G, int W>
+__global__ void __launch_bounds__(W * D / 8)
+kv4_write_kernel(Kv4 c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int bf16, int wide, int tokens, int64_t k_token,
+                 int64_t k_head, int64_t v_token, int64_t v_head, const int64_t* __restrict__ slots) {
+    constexpr int NG = D / G, LT = D / 8;
+    __shared__ __align__(16) uint8_t tiles[W * (D / 2)];
+    __shared__ uint16_t sides[4 * NG][W];
+    const int t = threadIdx.x / LT, l = threadIdx.x % LT, h = blockIdx.y;
+    const int64_t first = (int64_t)blockIdx.x * W;
+    const int here = (int)min((int64_t)W, tokens - first);
+    u4 raw[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int g = NG == 2 ? i : 0;
-        q[i] = bad[g] ? 0u : (uint32_t)fminf(fmaxf(rintf(x[i] / s[g] + z[g]), 0.f), 15.f);
+        const int64_t token = first + min(t, here - 1);
+        const uint16_t* src = (i ? v + token * v_token + h * v_head : k + token * k_token + h * k_head) + 8 * l;
+        if (wide) {
+            raw[i] = *reinterpret_cast<const u4*>(src);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) raw[i][j] = (uint32_t)src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
+        }
     }
-    const int page = (int)(slot / c.P), t = (int)(slot % c.P);
-    uint8_t* head = c.head(page, h);
-    if (live) {
-        const uint8_t byte = (uint8_t)(q[0] | (q[1] << 4));
-        if (value) head[kv4_value_tile<D>(c.P, t) + lane * 16 + kv4_place(t & 15)] = byte;
-        else head[kv4_key_row<D>(t) + lane] = byte;
+    const int64_t* const mine = slots + first;
+    const int64_t slot = t < here ? mine[t] : -1;
+    const bool live = slot >= 0 && slot < c.slots();
+    const uint64_t runs = kv4_runs<W>(mine, here, c.slots());
+    int at;
+    const int page = kv4_page(c, live ? slot : 0, at);
+    uint8_t* const head = c.head(page, h);
+    int start;
+    const int run = kv4_run_of(runs, t, start);
+
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        float x[8];
+        int nan = 0;
+        float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const uint32_t w = raw[i][j >> 1];
+            const float y = load16((j & 1 ? w >> 16 : w) & 0xFFFF, bf16);
+            nan |= y != y;
+            x[j] = fminf(fmaxf(y, -65504.f), 65504.f);
+            lo = fminf(lo, x[j]);
+            hi = fmaxf(hi, x[j]);
+        }
+        lo = over_lanes<G / 8>(lo, [](float p, float q) { return fminf(p, q); });
+        hi = over_lanes<G / 8>(hi, [](float p, float q) { return fmaxf(p, q); });
+        nan = over_lanes<G / 8>(nan, [](int p, int q) { return p | q; });
+        const float step = fmaxf(fmaxf((hi - lo) / 15.f, fmaxf(fabsf(lo), fabsf(hi)) / 96.f), 0x1p-14f);
+        const float s = half_bits(to_half_bits(step));
+        const float z = rintf(-lo / s * 8.f) / 8.f;
+        constexpr float kMagic = 8388608.f;                  // 2^23 + q has the code in its lowest byte
+        const float rs = __builtin_amdgcn_rcpf(s);
+        uint32_t q[8];
+        bool near = false;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = fminf(fmaxf(fmaf(x[j], rs, z), 0.f), 15.f), m = y + kMagic;
+            near |= fabsf(y - (m - kMagic)) > 0.5f - 0x1p-15f;
+            q[j] = __builtin_bit_cast(uint32_t, m);
+        }
+        if (near) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) q[j] = __builtin_bit_cast(uint32_t, fminf(fmaxf(rintf(x[j] / s + z), 0.f), 15.f) + kMagic);
+        }
+        uint32_t own[2];                                     // the eight codes as bytes
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const uint32_t a = __builtin_amdgcn_perm(q[4 * j + 1], q[4 * j], 0x0c0c0400u), b = __builtin_amdgcn_perm(q[4 * j + 3], q[4 * j + 2], 0x04000c0cu);
+            own[j] = nan ? 0u : a | b;
+        }
+        // the lane with the values D/2 further on has the upper codes
+        uint32_t both[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) both[j] = own[j] | ((uint32_t)dpp<kShiftDown + LT / 2>((int)own[j]) << 4);
+        if (l % (G / 8) == 0) {
+            sides[(2 * i) * NG + l / (G / 8)][t] = nan ? 0x7E00u : to_half_bits(s);
+            sides[(2 * i + 1) * NG + l / (G / 8)][t] = nan ? 0x7E00u : to_half_bits(z);
+        }
+        if (l >= LT / 2 || !live) continue;
+        if (i == 0) {
+            *reinterpret_cast<u2*>(head + kv4_key_row<D>(at) + 8 * l) = u2{both[0], both[1]};
+        } else {
+            uint8_t* to = run >= 0 ? tiles + run * (D / 2 * 16) + kv4_place(t - start) : head + kv4_value_tile<D>(c.P, at) + kv4_place(at & 15);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) to[(8 * l + j) * 16] = (uint8_t)(both[j >> 2] >> (8 * (j & 3)));
+        }
     }
-    if (lane < NG) {
-        const int g = lane;
-        const bool b = g == 0 ? bad[0] : bad[NG - 1];
-        const float sg = g == 0 ? s[0] : s[NG - 1], zg = g == 0 ? z[0] : z[NG - 1];
-        *reinterpret_cast<uint16_t*>(head + kv4_side<D, G>(c.P, value ? kValueScale : kKeyScale, g, t)) = b ? 0x7E00u : to_half_bits(sg);
-        *reinterpret_cast<uint16_t*>(head + kv4_side<D, G>(c.P, value ? kValueZero : kKeyZero, g, t)) = b ? 0x7E00u : to_half_bits(zg);
+    __syncthreads();
+    if (threadIdx.x < W / 16 * (D / 2)) {
+        const int which = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
+        if (which < __popcll(runs)) {
+            int in;
+            const int pg = kv4_page(c, mine[kv4_run_start(runs, which)], in);
+            *reinterpret_cast<u4*>(c.head(pg, h) + kv4_value_tile<D>(c.P, in) + j * 16) =
+                *reinterpret_cast<const u4*>(tiles + (which * (D / 2) + j) * 16);
+        }
+    }
+    if (threadIdx.x < 4 * NG * W) {
+        const int which = threadIdx.x / W, i = threadIdx.x % W;
+        const int64_t to = i < here ? mine[i] : -1;
+        if (to >= 0 && to < c.slots()) {
+            int in;
+            const int pg = kv4_page(c, to, in);
+            *reinterpret_cast<uint16_t*>(c.head(pg, h) + kv4_side<D, G>(c.P, which / NG, which % NG, in)) = sides[which][i];
+        }
     }
 }
 
-template <int D, int G>
-__global__ void __launch_bounds__(256)
+// Lane l of a token gives values 8 l .. 8 l + 7: the lower codes of eight bytes, or (from D/2 on) the upper ones of the same.
+template <int D, int G, int W>
+__global__ void __launch_bounds__(W * D / 8)
 kv4_read_kernel(Kv4 c, const int64_t* __restrict__ slots, int tokens, int bf16, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
-    const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int64_t token = unit / c.H;
-    const int h = (int)(unit % c.H);
-    if (token >= tokens || lane >= D / 2) return;
-    const bool value = blockIdx.y != 0;
-    const int64_t slot = slots[token];
-    uint16_t* dst = (value ? v : k) + unit * D;
-    if (slot < 0 || slot >= c.slots()) {
-        dst[lane] = dst[lane + D / 2] = 0;
-        return;
+    constexpr int LT = D / 8, PITCH = D / 2 + 8;
+    __shared__ __align__(16) uint8_t rows[W * PITCH];        // value codes of whole runs, token by token
+    const int t = threadIdx.x / LT, l = threadIdx.x % LT, h = blockIdx.y;
+    const int64_t first = (int64_t)blockIdx.x * W;
+    const int here = (int)min((int64_t)W, tokens - first);
+    const int64_t* const mine = slots + first;
+    const int64_t slot = t < here ? mine[t] : -1;
+    const bool live = slot >= 0 && slot < c.slots();
+    const uint64_t runs = kv4_runs<W>(mine, here, c.slots());
+    int at;
+    const int page = kv4_page(c, live ? slot : 0, at);
+    const uint8_t* const head = c.head(page, h);
+    int start;
+    const int run = kv4_run_of(runs, t, start), byte = 8 * l % (D / 2), g = l / (G / 8);
+    u2 w[2] = {{0, 0}, {0, 0}};
+    float s[2] = {0.f, 0.f}, z[2] = {0.f, 0.f};
+    if (live) {
+        w[0] = *reinterpret_cast<const u2*>(head + kv4_key_row<D>(at) + byte);
+        if (run < 0) {
+            const uint8_t* from = head + kv4_value_tile<D>(c.P, at) + kv4_place(at & 15) + byte * 16;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) w[1][j >> 2] |= (uint32_t)from[16 * j] << (8 * (j & 3));
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            s[i] = half_bits(*reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, i ? kValueScale : kKeyScale, g, at)));
+            z[i] = half_bits(*reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, i ? kValueZero : kKeyZero, g, at)));
+        }
     }
-    const int page = (int)(slot / c.P), t = (int)(slot % c.P);
-    const uint8_t* head = c.head(page, h);
-    const uint32_t byte = value ? head[kv4_value_tile<D>(c.P, t) + lane * 16 + kv4_place(t & 15)] : head[kv4_key_row<D>(t) + lane];
+    if (threadIdx.x < W / 16 * (D / 2)) {
+        const int which = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
+        if (which < __popcll(runs)) {                        // the same for the four lanes that exchange bytes
+            int in;
+            const int pg = kv4_page(c, mine[kv4_run_start(runs, which)], in);
+            const u4 w = *reinterpret_cast<const u4*>(c.head(pg, h) + kv4_value_tile<D>(c.P, in) + j * 16);
+            const uint32_t quad_a = j & 1 ? 0x03070105u : 0x06020400u, quad_b = j & 2 ? 0x03020706u : 0x05040100u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                    // bytes of four tokens -> this lane's token's byte of four lanes
+                uint32_t d = w[i];
+                d = __builtin_amdgcn_perm((uint32_t)dpp<kXor1>((int)d), d, quad_a);
+                d = __builtin_amdgcn_perm((uint32_t)dpp<kXor2>((int)d), d, quad_b);
+                *reinterpret_cast<uint32_t*>(rows + (which * 16 + 4 * i + kv4_place(j & 3)) * PITCH + (j & ~3)) = d;
+            }
+        }
+    }
+    __syncthreads();
+    if (t >= here) return;
+    if (run >= 0) w[1] = *reinterpret_cast<const u2*>(rows + (run * 16 + t - start) * PITCH + byte);
+    const int shift = l >= LT / 2 ? 4 : 0;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-        const int d = lane + i * (D / 2);
-        const float s = half_bits(*reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, value ? kValueScale : kKeyScale, d / G, t)));
-        const float z = half_bits(*reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, value ? kValueZero : kKeyZero, d / G, t)));
-        float x = ((float)((byte >> (4 * i)) & 15u) - z) * s;
-        asm("" : "+v"(x));      // the product, then its rounding: fused into one mixed FMA with +0, -0 would become +0
-        dst[d] = store16(x, bf16);
+        u4 out;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t u = w[i][j >> 1] >> (shift + 16 * (j & 1));
+            float x0 = ((float)(u & 15u) - z[i]) * s[i], x1 = ((float)((u >> 8) & 15u) - z[i]) * s[i];
+            // the products, then their rounding: fused into one mixed FMA with +0, -0 would become +0
+            asm("" : "+v"(x0), "+v"(x1));
+            out[j] = (uint32_t)store16(x0, bf16) | ((uint32_t)store16(x1, bf16) << 16);
+        }
+        *reinterpret_cast<u4*>((i ? v : k) + ((first + t) * c.H + h) * D + 8 * l) = out;
     }
 }
 
@@ -102,15 +239,15 @@ const char* kv4_check(const w4a16_kv4_cache* c) {
     if (c->group_size > c->head_dim) return "the group size must divide the head size";
     if (c->page_size < 16 || c->page_size > 4096 || c->page_size % 16 != 0) return "the page size must be a multiple of 16, 16..4096";
     if (c->kv_heads < 1 || c->kv_heads > 1024) return "kv_heads must be 1..1024";
-    if (c->pages < 0 || c->pages >= (int64_t)1 << 31) return "dimensions out of range";
+    if (c->pages < 0 || c->pages >= (int64_t)1 << 31 || c->pages * c->page_size >= (int64_t)1 << 35) return "dimensions out of range";
     if (c->pages > 0 && !c->data) return "null pointer";
     if (reinterpret_cast<uintptr_t>(c->data) % 16 != 0) return "the cache must be 16-byte aligned";
     return nullptr;
 }
 
 Kv4 kv4_of(const w4a16_kv4_cache* c) {
-    return Kv4{(uint8_t*)c->data, w4a16_kv4_page_bytes(c->page_size, c->head_dim, c->group_size), (int)c->pages, (int)c->page_size,
-               (int)c->kv_heads};
+    const uint32_t bytes = (uint32_t)w4a16_kv4_page_bytes(c->page_size, c->head_dim, c->group_size);
+    return Kv4{(uint8_t*)c->data, bytes, bytes * (uint32_t)c->kv_heads, (int)c->pages, (int)c->page_size, (int)c->kv_heads};
 }
 
 int kv4_fail(int code, const char* who, const char* what) {
@@ -118,6 +255,18 @@ int kv4_fail(int code, const char* who, const char* what) {
     snprintf(msg, sizeof(msg), "%s: %s", who, what);
     w4a16_set_last_error(msg);
     return code;
+}
+
+// Calls f with the cache's sizes and the window: 64 tokens where that still gives every CU a workgroup, else 16.
+template <class F>
+static void kv4_windows(const w4a16_kv4_cache* c, int64_t tokens, F f) {
+    kv4_sizes(c, [&](auto d, auto g) {
+        auto with = [&](auto w) {
+            f(d, g, w, dim3((unsigned)((tokens + w.value - 1) / w.value), (unsigned)c->kv_heads), dim3(w.value * d.value / 8));
+        };
+        if (tokens * c->kv_heads >= 256 * 64) with(std::integral_constant<int, 64>{});
+        else with(std::integral_constant<int, 16>{});
+    });
 }
 
 }  // namespace w4a16
@@ -140,10 +289,12 @@ extern "C" int w4a16_kv4_write(const w4a16_kv4_cache* cache, const void* k, cons
     if (!k || !v || !slots) return kv4_fail(W4A16_ERR_INVALID, "kv4_write", "null pointer");
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 2 != 0 || reinterpret_cast<uintptr_t>(slots) % 8 != 0)
         return kv4_fail(W4A16_ERR_INVALID, "kv4_write", "k and v must be 2-byte aligned, slots 8-byte aligned");
-    const dim3 grid((unsigned)((tokens * cache->kv_heads + 3) / 4), 2);
-    kv4_sizes(cache, [&](auto d, auto g) {
-        hipLaunchKernelGGL((kv4_write_kernel<d.value, g.value>), grid, dim3(256), 0, (hipStream_t)stream, kv4_of(cache), (const uint16_t*)k,
-                           (const uint16_t*)v, bf16, (int)tokens, k_token_stride, k_head_stride, v_token_stride, v_head_stride, slots);
+    const bool wide = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 && k_token_stride % 8 == 0 &&
+                      k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0;
+    kv4_windows(cache, tokens, [&](auto d, auto g, auto w, dim3 grid, dim3 block) {
+        hipLaunchKernelGGL((kv4_write_kernel<d.value, g.value, w.value>), grid, block, 0, (hipStream_t)stream, kv4_of(cache),
+                           (const uint16_t*)k, (const uint16_t*)v, bf16, wide, (int)tokens, k_token_stride, k_head_stride, v_token_stride,
+                           v_head_stride, slots);
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_write", hipGetErrorString(e));
     return W4A16_OK;
@@ -158,10 +309,9 @@ extern "C" int w4a16_kv4_read(const w4a16_kv4_cache* cache, const int64_t* slots
     if (!k || !v || !slots) return kv4_fail(W4A16_ERR_INVALID, "kv4_read", "null pointer");
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0 || reinterpret_cast<uintptr_t>(slots) % 8 != 0)
         return kv4_fail(W4A16_ERR_INVALID, "kv4_read", "k and v must be 16-byte aligned, slots 8-byte aligned");
-    const dim3 grid((unsigned)((tokens * cache->kv_heads + 3) / 4), 2);
-    kv4_sizes(cache, [&](auto d, auto g) {
-        hipLaunchKernelGGL((kv4_read_kernel<d.value, g.value>), grid, dim3(256), 0, (hipStream_t)stream, kv4_of(cache), slots, (int)tokens,
-                           bf16, (uint16_t*)k, (uint16_t*)v);
+    kv4_windows(cache, tokens, [&](auto d, auto g, auto w, dim3 grid, dim3 block) {
+        hipLaunchKernelGGL((kv4_read_kernel<d.value, g.value, w.value>), grid, block, 0, (hipStream_t)stream, kv4_of(cache), slots,
+                           (int)tokens, bf16, (uint16_t*)k, (uint16_t*)v);
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_read", hipGetErrorString(e));
     return W4A16_OK;

@@ -23,16 +23,7 @@ __device__ __forceinline__ void kv4_finish(const Kv4Attn& a, int64_t row, int d,
 
 typedef int i4v __attribute__((ext_vector_type(4)));
 
-// All-lane results over the 16 lanes of a row: neighbours, pairs, quads, halves.
-template <int CTRL>
-__device__ __forceinline__ int dpp(int v) {
-    return __builtin_amdgcn_mov_dpp(v, CTRL, 0xF, 0xF, true);
-}
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(int, v)));
-}
-constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
+// All-lane results over the 16 lanes of a row.
 #define W4A16_OVER_ROW(v, op)              \
     do {                                   \
         v = op(v, dpp<kXor1>(v));          \
@@ -57,15 +48,6 @@ __device__ __forceinline__ float of_digits4(int d0, int d1, int d2, int d3) {
     return fmaf((float)((d3 << 8) + d2), 65536.f, (float)((d1 << 8) + d0));
 }
 
-// Keys and values of 64 tokens in flight, for lane (kb, n) = (lane / 16, lane % 16).
-template <int D, int NG>
-struct KvTile {
-    u4 k[4];                                 // 16 bytes of the row of token 16 r + n
-    u4 v[D / 32];                            // tokens 16 kb .. + 15 of byte n + 16 i
-    uint16_t side[4][NG];                    // of token 16 kb + n
-    bool there;                              // the page of tokens 16 kb .. + 15 is in the cache
-};
-
 // One workgroup takes one KV head of one sequence and a share of its tiles of 64 keys, a wave one tile at a time;
 // 4 NT rows (query, query head) at once.  Both products run on v_mfma_i32_16x16x64_i8: the codes are its operand as
 // they lie in the cache (one mask, for the upper codes one shift), the other operand is a fixed-point number in
@@ -75,7 +57,7 @@ struct KvTile {
 // The integer sums are exact, those of 8 z_t (in two digits, one more column of the product) among them, and are taken
 // off digit by digit: a value that is 0 weighs nothing however large p is.  The digits come together in fp32.  Per 64 keys a wave issues about 300 vector
 // instructions for 8.7 KB, under a third of the time that HBM takes to bring them.
-template <int D, int G, int NT, int WAVES>
+template <int D, int G, int NT, int WAVES, bool ONE>
 __global__ void __launch_bounds__(64 * WAVES)
 kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
                  float* __restrict__ part_o) {
@@ -84,18 +66,22 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
     constexpr int kSide = NG * (64 * 8 + 128), kDigits = NT * NG * 1024;
     constexpr int kLoop = WAVES * (kSide + kDigits), kJoin = WAVES * 4 * NT * (D + 2) * 4;
     __shared__ __align__(16) uint8_t lds[kLoop > kJoin ? kLoop : kJoin];
-    const int lane = threadIdx.x & 63, kb = lane >> 4, n = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint8_t* const side = lds + wave * (kSide + kDigits);
     uint8_t* const dig = side + kSide;
     const int h = blockIdx.x % a.c.H, split = blockIdx.x / a.c.H, b = blockIdx.y;
     const Kv4Seq s = kv4_seq(a, b);
-    const int rows = s.count * a.rep, base = s.len - s.count, groups = a.c.P >> 4;
+    const int rows = s.count * a.rep, base = s.len - s.count;
+    const int units = ONE ? a.c.P >> 6 : a.c.P >> 4;         // tiles, or groups of 16 tokens, of a page
     const int* const table = a.table + b * a.table_stride;
-    const uint32_t quad_a = lane & 1 ? 0x03070105u : 0x06020400u;   // selectors of the 4 x 4 byte transpose below
-    const uint32_t quad_b = lane & 2 ? 0x03070206u : 0x05010400u;
+    const uint8_t* const mine = a.c.data + (uint64_t)(uint32_t)h * a.c.head_bytes;      // this head's bytes of page 0
 
     for (int row0 = 0; row0 < rows; row0 += 4 * NT) {
+        int lane = threadIdx.x & 63;
+        asm volatile("" : "+v"(lane));                       // what follows from it is not kept in registers across passes
+        const int kb = lane >> 4, n = lane & 15;
+        const uint32_t quad_a = lane & 1 ? 0x03070105u : 0x06020400u;   // selectors of the 4 x 4 byte transpose below
+        const uint32_t quad_b = lane & 2 ? 0x03070206u : 0x05010400u;
         const int first = row0 / a.rep, last = (min(row0 + 4 * NT, rows) - 1) / a.rep;
         const int kmax = a.causal ? max(0, min(base + last + 1, s.len)) : s.len;
         const int kmin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
@@ -169,9 +155,9 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                 const int sum = NG == 2 || D == 64 ? sums[g] : sums[0] + sums[D / 64 - 1];
                 qsum[t][g] = (float)__shfl(sum, 4 * kb, 64);
             }
-            rs[t] = __shfl(finite ? ldexpf(a.scale2, e - 22) : NAN, 4 * kb, 64);
-            const int mine = row0 + 4 * t + kb, pos = base + mine / a.rep;
-            end[t] = mine < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
+            rs[t] = __shfl(finite ? fmaxf(ldexpf(a.scale2, e - 22), 0x1p-126f) : NAN, 4 * kb, 64);
+            const int own = row0 + 4 * t + kb, pos = base + own / a.rep;
+            end[t] = own < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
             begin[t] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
         }
 
@@ -186,55 +172,71 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             for (int i = 0; i < NV; ++i) o[t][0][i] = o[t][1][i] = 0.f;
         }
 
-        // A tile's page and place in it for the lane's 16 tokens: the table entry comes one tile ahead of the tile
-        auto entry = [&](int tile) {
-            const int group = tile * 4 + kb;
-            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
-            return group * 16 < kmax ? table[at] : -1;
+        // What a lane holds of a tile of 64 tokens.  Each part of the next tile is sent for where this tile's has been used.
+        u4 k[4];                                             // 16 bytes of the row of token 16 r + n
+        u4 v[NV];                                            // tokens 16 kb .. + 15 of byte n + 16 i
+        uint16_t sides[4][NG];                               // of token 16 kb + n
+        // Where they come from: the page's bytes of this head and the place in it of the tile (ONE: every tile lies in one
+        // page, so for the whole wave) or of tokens 16 kb .. + 15 (for the lane)
+        bool there = false;                                  // the page is in the cache
+        uint64_t kv = 0;
+        int place = 0;
+        auto entry_at = [&](int tile) {
+            const int unit = ONE ? tile : tile * 4 + kb;
+            return units == 1 ? unit : (int)__umulhi((uint32_t)unit, page_magic);
         };
-        auto load = [&](int tile, int page, KvTile<D, NG>& x) {
-            const int group = tile * 4 + kb;
-            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
-            const int place = (group - at * groups) * 16;
-            x.there = (uint32_t)page < (uint32_t)a.c.pages;
-            const int pg = x.there ? page : 0;
-            const uint8_t* mine = a.c.head(pg, h);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const uint8_t* row = a.c.head(__builtin_amdgcn_readlane(pg, 16 * r), h) + kv4_key_row<D>(__builtin_amdgcn_readlane(place, 16 * r));
-                x.k[r] = *reinterpret_cast<const u4*>(row + n * (D / 2) + 16 * (D == 128 ? kb : kb & 1));
-            }
-            const uint8_t* vals = mine + kv4_value_tile<D>(a.c.P, place) + n * 16;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) x.v[i] = *reinterpret_cast<const u4*>(vals + 256 * i);
+        auto entry = [&](int tile) { return ONE || tile * 64 + kb * 16 < kmax ? table[entry_at(tile)] : -1; };
+        auto aim = [&](int tile, int page) {
+            place = ONE ? (tile - entry_at(tile) * units) * 64 : (tile * 4 + kb - entry_at(tile) * units) * 16;
+            there = (uint32_t)page < (uint32_t)a.c.pages;
+            kv = (uint64_t)(uint32_t)(there ? page : 0) * a.c.page_bytes;
+        };
+        auto load_sides = [&] {
+            const uint8_t* at = mine + kv + place * 2;
 #pragma unroll
             for (int w = 0; w < 4; ++w)
 #pragma unroll
                 for (int g = 0; g < NG; ++g)
-                    x.side[w][g] = *reinterpret_cast<const uint16_t*>(mine + kv4_side<D, G>(a.c.P, w, g, place + n));
+                    sides[w][g] = *reinterpret_cast<const uint16_t*>(at + kv4_side<D, G>(a.c.P, w, g, 0) + (uint32_t)((ONE ? lane : n) * 2));
+        };
+        auto load_keys = [&] {
+            const uint64_t at = kv + kv4_key_row<D>(place);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t in = n * (D / 2) + 16 * (D == 128 ? kb : kb & 1);
+                uint64_t row = at + r * 16 * (D / 2);
+                if constexpr (!ONE)
+                    row = ((uint64_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), 16 * r) << 32) |
+                          __builtin_amdgcn_readlane((uint32_t)at, 16 * r);
+                k[r] = *reinterpret_cast<const u4*>(mine + row + in);
+            }
+        };
+        auto load_values = [&] {
+            const uint8_t* vals = mine + kv + kv4_value_tile<D>(a.c.P, place);
+            const uint32_t in = n * 16 + (ONE ? kb * (D / 2 * 16) : 0);
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const u4*>(vals + in + 256 * i);
         };
 
         const int stop = tile0 + min(tiles, (split + 1) * per);
-        int tile = tile0 + split * per + wave;
-        KvTile<D, NG> x;
-        int next_page = -1;
+        int tile = tile0 + split * per + wave, page = -1;
         if (tile < stop) {
-            load(tile, entry(tile), x);
-            if (tile + WAVES < stop) next_page = entry(tile + WAVES);
+            aim(tile, entry(tile));
+            load_sides();
+            load_keys();
+            load_values();
+            if (tile + WAVES < stop) page = entry(tile + WAVES);
         }
         for (; tile < stop; tile += WAVES) {
-            const KvTile<D, NG> c = x;
-            if (tile + WAVES < stop) {
-                load(tile + WAVES, next_page, x);
-                if (tile + 2 * WAVES < stop) next_page = entry(tile + 2 * WAVES);
-            }
+            const bool more = tile + WAVES < stop, here = there;
             // scales and zeros through LDS, nothing for tokens that no row sees; the largest value scale
-            const bool live = c.there && tile * 64 + lane < kmax;
+            const bool live = here && tile * 64 + lane < kmax;
             uint32_t big = 0;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                u2 w = u2{(uint32_t)c.side[kKeyScale][g] | ((uint32_t)c.side[kKeyZero][g] << 16), c.side[kValueScale][g]};
-                int z = (int)(half_bits(c.side[kValueZero][g]) * 8.f);
+                // scales together with the key zeros; the value zeros, eightfold, as two digits
+                u2 w = u2{(uint32_t)sides[kKeyScale][g] | ((uint32_t)sides[kKeyZero][g] << 16), sides[kValueScale][g]};
+                int z = (int)(half_bits(sides[kValueZero][g]) * 8.f);
                 if (!live) {
                     w = u2{0, 0};
                     z = 0;
@@ -243,7 +245,12 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                 uint8_t* const zb = side + NG * 512 + g * 128 + kb * 32 + kv4_place(n);
                 zb[0] = (uint8_t)(z & 15);
                 zb[16] = (uint8_t)(z >> 4);
-                big = max(big, min(w.y, 0x7BFFu));
+                big = max(big, w.y);
+            }
+            if (more) {
+                aim(tile + WAVES, page);
+                load_sides();
+                if (tile + 2 * WAVES < stop) page = entry(tile + 2 * WAVES);
             }
             {
                 int v = (int)big;
@@ -252,7 +259,8 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                                     max(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
             }
             // every value scale is under 2^(ev - 14), p s in units of 2^(ev - 44) under 2^30
-            const int ev = (int)(big >> 10);
+            const bool odd = big > 0x7BFFu;                  // a scale that is no number
+            const int ev = (int)(min(big, 0x7BFFu) >> 10);
             const float unit = __builtin_bit_cast(float, (uint32_t)(127 + 44 - ev) << 23);
             const float back = __builtin_bit_cast(float, (uint32_t)(127 - 47 + ev) << 23);
             const bool whole = __all(live) && tile * 64 + 64 <= sure_end && tile * 64 >= sure_begin;
@@ -270,7 +278,7 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                     zk[g] = half_bits(w0 >> 16);
                     sv[r][g] = half_bits(w1 & 0xFFFF);
                 }
-                const u4 w = c.k[r];
+                const u4 w = k[r];
                 i4v code[D / 64];
                 if constexpr (D == 128) {
                     code[0] = __builtin_bit_cast(i4v, w & 0x0F0F0F0Fu);
@@ -289,9 +297,11 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                     float y = 0.f;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) y += fmaf(-zk[g], qsum[t][g], of_digits3(dot[g][0], dot[g][1], dot[g][2])) * sk[g];
-                    sc[t][r] = y * rs[t];
+                    sc[t][r] = y;                            // times rs
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);               // not before this tile's are used: they take their registers
+            if (more) load_keys();
             i4v pd[NT][NG];
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
@@ -300,30 +310,34 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const int at = tile * 64 + 16 * r + n;
-                        see[r] = __builtin_amdgcn_readlane((int)c.there, 16 * r) && at < end[t] && at >= begin[t];
+                        see[r] = __builtin_amdgcn_readlane((int)here, 16 * r) && at < end[t] && at >= begin[t];
                         if (!see[r]) sc[t][r] = -INFINITY;
                     }
                 }
                 float top = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]));
                 W4A16_OVER_ROW(top, fmaxf);
-                const float next = fmaxf(m[t], top), safe = next == -INFINITY ? 0.f : next;
-                const float keep = __builtin_amdgcn_exp2f(m[t] - safe);
-                m[t] = next;
-                l[t] *= keep;
+                top *= rs[t];
+                if (__any(top > m[t])) {
+                    const float next = fmaxf(m[t], top);     // above -inf where m is
+                    const float keep = next == m[t] ? 1.f : __builtin_amdgcn_exp2f(m[t] - next);
+                    m[t] = next;
+                    l[t] *= keep;
 #pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    o[t][0][i] *= keep;
-                    o[t][1][i] *= keep;
+                    for (int i = 0; i < NV; ++i) {
+                        o[t][0][i] *= keep;
+                        o[t][1][i] *= keep;
+                    }
                 }
+                const float safe = m[t] == -INFINITY ? 0.f : -m[t];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(sc[t][r] - safe);
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][r], rs[t], safe));
                     l[t] += p;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         float ps = p * sv[r][g];
                         if (!whole && !see[r]) ps = 0.f;            // a token that another row sees may hold NaN
-                        nan[t][g] = fmaf(ps, 0.f, nan[t][g]);
+                        if (odd) nan[t][g] = fmaf(ps, 0.f, nan[t][g]);
                         // four neighbouring lanes exchange bytes so that lane i of them holds digit i of their tokens
                         uint32_t d = digits4((int)(ps * unit));
                         d = __builtin_amdgcn_perm((uint32_t)dpp<kXor1>((int)d), d, quad_a);
@@ -337,9 +351,9 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             for (int t = 0; t < NT; ++t)
 #pragma unroll
                 for (int g = 0; g < NG; ++g) pd[t][g] = *reinterpret_cast<const i4v*>(dig + (t * NG + g) * 1024 + kb * 256 + n * 16);
-            // sums of digits times 8 z: even columns hold those of its low digit, odd ones of its high
-            int cz[NT][NG][4];
-            const int low = n & 1 ? 16 : 1, high = n & 1 ? 1 : 16;
+            // less the sums of digits times 8 z: even columns hold those of its low digit, odd ones of its high
+            i4v less[NT][NG];
+            const int low = n & 1 ? -16 : -1, high = n & 1 ? -1 : -16;
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
                 const i4v zb = *reinterpret_cast<const i4v*>(side + NG * 512 + g * 128 + kb * 32 + (n & 1) * 16);
@@ -348,28 +362,23 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                     const i4v none = {0, 0, 0, 0};
                     const i4v y = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][g], zb, none, 0, 0, 0);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) cz[t][g][i] = __mul24(y[i], low) + __mul24(dpp<kXor1>(y[i]), high);
+                    for (int i = 0; i < 4; ++i) less[t][g][i] = __mul24(y[i], low) + __mul24(dpp<kXor1>(y[i]), high);
                 }
             }
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const u4 w = c.v[i];
-                const i4v lo = __builtin_bit_cast(i4v, w & 0x0F0F0F0Fu), hi = __builtin_bit_cast(i4v, (w >> 4) & 0x0F0F0F0Fu);
+                const u4 w = v[i];                           // the codes eightfold, to go with 8 z
+                const i4v lo = __builtin_bit_cast(i4v, (w << 3) & 0x78787878u), hi = __builtin_bit_cast(i4v, (w >> 1) & 0x78787878u);
 #pragma unroll
                 for (int t = 0; t < NT; ++t) {
-                    const i4v none = {0, 0, 0, 0};
-                    const i4v y0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][0], lo, none, 0, 0, 0);
-                    const i4v y1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][NG - 1], hi, none, 0, 0, 0);
-                    int e0[4], e1[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        e0[j] = (y0[j] << 3) - cz[t][0][j];
-                        e1[j] = (y1[j] << 3) - cz[t][NG - 1][j];
-                    }
-                    o[t][0][i] = fmaf(of_digits4(e0[0], e0[1], e0[2], e0[3]), back, o[t][0][i]);
-                    o[t][1][i] = fmaf(of_digits4(e1[0], e1[1], e1[2], e1[3]), back, o[t][1][i]);
+                    const i4v y0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][0], lo, less[t][0], 0, 0, 0);
+                    const i4v y1 = __builtin_amdgcn_mfma_i32_16x16x64_i8(pd[t][NG - 1], hi, less[t][NG - 1], 0, 0, 0);
+                    o[t][0][i] = fmaf(of_digits4(y0[0], y0[1], y0[2], y0[3]), back, o[t][0][i]);
+                    o[t][1][i] = fmaf(of_digits4(y1[0], y1[1], y1[2], y1[3]), back, o[t][1][i]);
                 }
             }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_values();
         }
 
         // The waves' shares come together in LDS
@@ -396,8 +405,8 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
         }
         __syncthreads();
         for (int i = threadIdx.x; i < 4 * NT * (D / 2); i += 64 * WAVES) {
-            const int r = i / (D / 2), d = i % (D / 2) * 2, mine = row0 + r;
-            if (mine >= rows) continue;
+            const int r = i / (D / 2), d = i % (D / 2) * 2, own = row0 + r;
+            if (own >= rows) continue;
             float top = jm[r];
 #pragma unroll
             for (int w = 1; w < WAVES; ++w) top = fmaxf(top, jm[w * 4 * NT + r]);
@@ -411,7 +420,7 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
                 v0 = fmaf(f, y.x, v0);
                 v1 = fmaf(f, y.y, v1);
             }
-            const int64_t row = (int64_t)(s.first + mine / a.rep) * a.heads + h * a.rep + mine % a.rep;
+            const int64_t row = (int64_t)(s.first + own / a.rep) * a.heads + h * a.rep + own % a.rep;
             if (parts == 1) {
                 kv4_finish<D>(a, row, d, top, sum, v0, v1);
                 if (used && d == 0) used[row] = 1;
@@ -929,11 +938,18 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
     float2* const ml = (float2*)(ws + plan.ml_at);
     float* const po = (float*)(ws + plan.o_at);
     kv4_sizes(cache, [&](auto d, auto g) {
-        const uint32_t magic = (uint32_t)(((uint64_t)1 << 32) / (uint64_t)(cache->page_size / 16) + 1);
+        auto magic_of = [](int64_t n) { return (uint32_t)(((uint64_t)1 << 32) / (uint64_t)n + 1); };      // u / n = mulhi(u, that), n > 1
         if (plan.nt) {
+            const bool one = cache->page_size % 64 == 0;     // no tile of 64 tokens crosses a page
+            const uint32_t magic = magic_of(cache->page_size / (one ? 64 : 16));
             const dim3 grid((unsigned)(cache->kv_heads * plan.splits), (unsigned)args->batch);
             auto launch = [&](auto nt) {
-                hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4>), grid, dim3(256), 0, st, a, plan.splits, magic, used, ml, po);
+                if (one)
+                    hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4, true>), grid, dim3(256), 0, st, a, plan.splits, magic,
+                                       used, ml, po);
+                else
+                    hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4, false>), grid, dim3(256), 0, st, a, plan.splits, magic,
+                                       used, ml, po);
             };
             if (plan.nt == 1) launch(std::integral_constant<int, 1>{});
             else if (plan.nt == 2) launch(std::integral_constant<int, 2>{});
@@ -941,7 +957,7 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
         } else {
             const dim3 grid((unsigned)cache->kv_heads, (unsigned)(plan.row_tiles * plan.splits), (unsigned)args->batch);
             hipLaunchKernelGGL((kv4_prompt_kernel<d.value, g.value, kPromptWaves>), grid, dim3(64 * kPromptWaves), 0, st, a, plan.row_tiles,
-                               plan.splits, magic, used, ml, po);
+                               plan.splits, magic_of(cache->page_size / 16), used, ml, po);
         }
         if (plan.splits > 1)
             hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits, used,
