@@ -1,6 +1,8 @@
 // Writing keys and values into the 4-bit cache and reading them back (include/w4a16.h has the format).
 #include <stdio.h>
 
+#include <algorithm>
+
 #include "w4a16_internal.h"
 #include "w4a16_kv4.h"
 
@@ -53,181 +55,202 @@ __device__ __forceinline__ T over_lanes(T v, F f) {
 // Every operation is an IEEE fp32 operation or agrees with one, so the bytes are the format's definition.  The codes'
 // quotient x / s is taken as x rcp(s) first: with |x / s| < 113 the two differ by less than 2^-16, so only a value
 // whose x rcp(s) + z is within 2^-15 of a half-integer needs the division.
-template <int D, int G, int W>
+template <int D, int G, int W, bool BF16>
 __global__ void __launch_bounds__(W * D / 8)
-kv4_write_kernel(Kv4 c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int bf16, int wide, int tokens, int64_t k_token,
+kv4_write_kernel(Kv4 c, const uint16_t* __restrict__ k, const uint16_t* __restrict__ v, int wide, int tokens, int64_t k_token,
                  int64_t k_head, int64_t v_token, int64_t v_head, const int64_t* __restrict__ slots) {
     constexpr int NG = D / G, LT = D / 8;
     __shared__ __align__(16) uint8_t tiles[W * (D / 2)];
     __shared__ uint16_t sides[4 * NG][W];
-    const int t = threadIdx.x / LT, l = threadIdx.x % LT, h = blockIdx.y;
+    const int t = threadIdx.x / LT, l = threadIdx.x % LT;
     const int64_t first = (int64_t)blockIdx.x * W;
     const int here = (int)min((int64_t)W, tokens - first);
+    const int64_t token = first + min(t, here - 1);
+    const uint16_t* src[2] = {k + token * k_token + 8 * l, v + token * v_token + 8 * l};
     u4 raw[2];
+    auto load = [&](int h) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int64_t token = first + min(t, here - 1);
-        const uint16_t* src = (i ? v + token * v_token + h * v_head : k + token * k_token + h * k_head) + 8 * l;
-        if (wide) {
-            raw[i] = *reinterpret_cast<const u4*>(src);
-        } else {
+        for (int i = 0; i < 2; ++i) {
+            const uint16_t* from = src[i] + h * (i ? v_head : k_head);
+            if (wide) {
+                raw[i] = *reinterpret_cast<const u4*>(from);
+            } else {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) raw[i][j] = (uint32_t)src[2 * j] | ((uint32_t)src[2 * j + 1] << 16);
+                for (int j = 0; j < 4; ++j) raw[i][j] = (uint32_t)from[2 * j] | ((uint32_t)from[2 * j + 1] << 16);
+            }
         }
-    }
+    };
+    load(blockIdx.y);
     const int64_t* const mine = slots + first;
     const int64_t slot = t < here ? mine[t] : -1;
     const bool live = slot >= 0 && slot < c.slots();
     const uint64_t runs = kv4_runs<W>(mine, here, c.slots());
-    int at;
-    const int page = kv4_page(c, live ? slot : 0, at);
-    uint8_t* const head = c.head(page, h);
-    int start;
+    int at, start;
+    uint8_t* const page = c.head(kv4_page(c, live ? slot : 0, at), 0);
     const int run = kv4_run_of(runs, t, start);
+    // what this thread stores for the window: 16 bytes of a run, and a scale or zero of a token
+    const int which = threadIdx.x / (D / 2), piece = threadIdx.x % (D / 2);
+    uint8_t* run_to = nullptr;
+    if (which < __popcll(runs)) {
+        int in;
+        uint8_t* const to = c.head(kv4_page(c, mine[kv4_run_start(runs, which)], in), 0);
+        run_to = to + kv4_value_tile<D>(c.P, in) + piece * 16;
+    }
+    const int part = threadIdx.x / W, i_side = threadIdx.x % W;
+    uint8_t* side_to = nullptr;
+    if (part < 4 * NG && i_side < here) {
+        const int64_t s = mine[i_side];
+        int in;
+        uint8_t* const to = c.head(kv4_page(c, s >= 0 && s < c.slots() ? s : 0, in), 0);
+        if (s >= 0 && s < c.slots()) side_to = to + kv4_side<D, G>(c.P, part / NG, part % NG, in);
+    }
 
+    for (int h = blockIdx.y; h < c.H; h += gridDim.y) {
+        const uint32_t head = (uint32_t)h * c.head_bytes;
+        const u4 now[2] = {raw[0], raw[1]};
+        if (h + (int)gridDim.y < c.H) load(h + gridDim.y);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        float x[8];
-        int nan = 0;
-        float lo = INFINITY, hi = -INFINITY;
+        for (int i = 0; i < 2; ++i) {
+            float x[8];
+            int nan = 0;
+            float lo = INFINITY, hi = -INFINITY, before = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const uint32_t w = raw[i][j >> 1];
-            const float y = load16((j & 1 ? w >> 16 : w) & 0xFFFF, bf16);
-            nan |= y != y;
-            x[j] = fminf(fmaxf(y, -65504.f), 65504.f);
-            lo = fminf(lo, x[j]);
-            hi = fmaxf(hi, x[j]);
-        }
-        lo = over_lanes<G / 8>(lo, [](float p, float q) { return fminf(p, q); });
-        hi = over_lanes<G / 8>(hi, [](float p, float q) { return fmaxf(p, q); });
-        nan = over_lanes<G / 8>(nan, [](int p, int q) { return p | q; });
-        const float step = fmaxf(fmaxf((hi - lo) / 15.f, fmaxf(fabsf(lo), fabsf(hi)) / 96.f), 0x1p-14f);
-        const float s = half_bits(to_half_bits(step));
-        const float z = rintf(-lo / s * 8.f) / 8.f;
-        constexpr float kMagic = 8388608.f;                  // 2^23 + q has the code in its lowest byte
-        const float rs = __builtin_amdgcn_rcpf(s);
-        uint32_t q[8];
-        bool near = false;
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t w = now[i][j >> 1];
+                const float y = load16((j & 1 ? w >> 16 : w) & 0xFFFF, BF16);
+                if (j & 1) nan |= __builtin_isunordered(y, before);
+                before = y;
+                x[j] = __builtin_amdgcn_fmed3f(y, -65504.f, 65504.f);
+                lo = fminf(lo, x[j]);
+                hi = fmaxf(hi, x[j]);
+            }
+            lo = over_lanes<G / 8>(lo, [](float p, float q) { return fminf(p, q); });
+            hi = over_lanes<G / 8>(hi, [](float p, float q) { return fmaxf(p, q); });
+            nan = over_lanes<G / 8>(nan, [](int p, int q) { return p | q; });
+            const float step = fmaxf(fmaxf((hi - lo) / 15.f, fmaxf(fabsf(lo), fabsf(hi)) / 96.f), 0x1p-14f);
+            const float s = half_bits(to_half_bits(step));
+            const float z = rintf(-lo / s * 8.f) / 8.f;
+            constexpr float kMagic = 8388608.f;              // 2^23 + q has the code in its lowest byte
+            const float rs = __builtin_amdgcn_rcpf(s);
+            uint32_t q[8];
+            float off = 0.f;                                 // how far the furthest value is from its code
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float y = fminf(fmaxf(fmaf(x[j], rs, z), 0.f), 15.f), m = y + kMagic;
-            near |= fabsf(y - (m - kMagic)) > 0.5f - 0x1p-15f;
-            q[j] = __builtin_bit_cast(uint32_t, m);
-        }
-        if (near) {
+            for (int j = 0; j < 8; ++j) {
+                const float y = __builtin_amdgcn_fmed3f(fmaf(x[j], rs, z), 0.f, 15.f), m = y + kMagic;
+                off = fmaxf(off, fabsf(y - (m - kMagic)));
+                q[j] = __builtin_bit_cast(uint32_t, m);
+            }
+            if (off > 0.5f - 0x1p-15f) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) q[j] = __builtin_bit_cast(uint32_t, fminf(fmaxf(rintf(x[j] / s + z), 0.f), 15.f) + kMagic);
-        }
-        uint32_t own[2];                                     // the eight codes as bytes
+                for (int j = 0; j < 8; ++j) q[j] = __builtin_bit_cast(uint32_t, fminf(fmaxf(rintf(x[j] / s + z), 0.f), 15.f) + kMagic);
+            }
+            // the eight codes as bytes; the lane with the values D/2 further on has the upper codes of the same bytes
+            uint32_t both[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const uint32_t a = __builtin_amdgcn_perm(q[4 * j + 1], q[4 * j], 0x0c0c0400u), b = __builtin_amdgcn_perm(q[4 * j + 3], q[4 * j + 2], 0x04000c0cu);
-            own[j] = nan ? 0u : a | b;
-        }
-        // the lane with the values D/2 further on has the upper codes
-        uint32_t both[2];
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t a = __builtin_amdgcn_perm(q[4 * j + 1], q[4 * j], 0x0c0c0400u);
+                const uint32_t own = nan ? 0u : a | __builtin_amdgcn_perm(q[4 * j + 3], q[4 * j + 2], 0x04000c0cu);
+                both[j] = own | ((uint32_t)dpp<kShiftDown + LT / 2>((int)own) << 4);
+            }
+            if (l % (G / 8) == 0) {
+                sides[(2 * i) * NG + l / (G / 8)][t] = nan ? 0x7E00u : to_half_bits(s);
+                sides[(2 * i + 1) * NG + l / (G / 8)][t] = nan ? 0x7E00u : to_half_bits(z);
+            }
+            if (l < LT / 2 && live) {
+                if (i == 0) {
+                    *reinterpret_cast<u2*>(page + head + kv4_key_row<D>(at) + 8 * l) = u2{both[0], both[1]};
+                } else if (run >= 0) {
 #pragma unroll
-        for (int j = 0; j < 2; ++j) both[j] = own[j] | ((uint32_t)dpp<kShiftDown + LT / 2>((int)own[j]) << 4);
-        if (l % (G / 8) == 0) {
-            sides[(2 * i) * NG + l / (G / 8)][t] = nan ? 0x7E00u : to_half_bits(s);
-            sides[(2 * i + 1) * NG + l / (G / 8)][t] = nan ? 0x7E00u : to_half_bits(z);
-        }
-        if (l >= LT / 2 || !live) continue;
-        if (i == 0) {
-            *reinterpret_cast<u2*>(head + kv4_key_row<D>(at) + 8 * l) = u2{both[0], both[1]};
-        } else {
-            uint8_t* to = run >= 0 ? tiles + run * (D / 2 * 16) + kv4_place(t - start) : head + kv4_value_tile<D>(c.P, at) + kv4_place(at & 15);
+                    for (int j = 0; j < 8; ++j) tiles[(run * (D / 2) + 8 * l + j) * 16 + kv4_place(t - start)] = (uint8_t)(both[j >> 2] >> (8 * (j & 3)));
+                } else {
+                    uint8_t* const to = page + head + kv4_value_tile<D>(c.P, at) + kv4_place(at & 15);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) to[(8 * l + j) * 16] = (uint8_t)(both[j >> 2] >> (8 * (j & 3)));
+                    for (int j = 0; j < 8; ++j) to[(8 * l + j) * 16] = (uint8_t)(both[j >> 2] >> (8 * (j & 3)));
+                }
+            }
         }
-    }
-    __syncthreads();
-    if (threadIdx.x < W / 16 * (D / 2)) {
-        const int which = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
-        if (which < __popcll(runs)) {
-            int in;
-            const int pg = kv4_page(c, mine[kv4_run_start(runs, which)], in);
-            *reinterpret_cast<u4*>(c.head(pg, h) + kv4_value_tile<D>(c.P, in) + j * 16) =
-                *reinterpret_cast<const u4*>(tiles + (which * (D / 2) + j) * 16);
-        }
-    }
-    if (threadIdx.x < 4 * NG * W) {
-        const int which = threadIdx.x / W, i = threadIdx.x % W;
-        const int64_t to = i < here ? mine[i] : -1;
-        if (to >= 0 && to < c.slots()) {
-            int in;
-            const int pg = kv4_page(c, to, in);
-            *reinterpret_cast<uint16_t*>(c.head(pg, h) + kv4_side<D, G>(c.P, which / NG, which % NG, in)) = sides[which][i];
-        }
+        __syncthreads();
+        if (run_to) *reinterpret_cast<u4*>(run_to + head) = *reinterpret_cast<const u4*>(tiles + threadIdx.x * 16);
+        if (side_to) *reinterpret_cast<uint16_t*>(side_to + head) = sides[part][i_side];
+        __syncthreads();
     }
 }
 
 // Lane l of a token gives values 8 l .. 8 l + 7: the lower codes of eight bytes, or (from D/2 on) the upper ones of the same.
-template <int D, int G, int W>
+// q - z is exact in fp16 (1024 + 16 q times 1/16 less 64 + z), and so its product with s needs one rounding.
+template <int D, int G, int W, bool BF16>
 __global__ void __launch_bounds__(W * D / 8)
-kv4_read_kernel(Kv4 c, const int64_t* __restrict__ slots, int tokens, int bf16, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
+kv4_read_kernel(Kv4 c, const int64_t* __restrict__ slots, int tokens, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
     constexpr int LT = D / 8, PITCH = D / 2 + 8;
     __shared__ __align__(16) uint8_t rows[W * PITCH];        // value codes of whole runs, token by token
-    const int t = threadIdx.x / LT, l = threadIdx.x % LT, h = blockIdx.y;
+    const int t = threadIdx.x / LT, l = threadIdx.x % LT;
     const int64_t first = (int64_t)blockIdx.x * W;
     const int here = (int)min((int64_t)W, tokens - first);
     const int64_t* const mine = slots + first;
     const int64_t slot = t < here ? mine[t] : -1;
     const bool live = slot >= 0 && slot < c.slots();
     const uint64_t runs = kv4_runs<W>(mine, here, c.slots());
-    int at;
-    const int page = kv4_page(c, live ? slot : 0, at);
-    const uint8_t* const head = c.head(page, h);
-    int start;
+    int at, start;
+    const uint8_t* const page = c.head(kv4_page(c, live ? slot : 0, at), 0);
     const int run = kv4_run_of(runs, t, start), byte = 8 * l % (D / 2), g = l / (G / 8);
-    u2 w[2] = {{0, 0}, {0, 0}};
-    float s[2] = {0.f, 0.f}, z[2] = {0.f, 0.f};
-    if (live) {
-        w[0] = *reinterpret_cast<const u2*>(head + kv4_key_row<D>(at) + byte);
-        if (run < 0) {
-            const uint8_t* from = head + kv4_value_tile<D>(c.P, at) + kv4_place(at & 15) + byte * 16;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) w[1][j >> 2] |= (uint32_t)from[16 * j] << (8 * (j & 3));
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            s[i] = half_bits(*reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, i ? kValueScale : kKeyScale, g, at)));
-            z[i] = half_bits(*reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, i ? kValueZero : kKeyZero, g, at)));
-        }
+    const int which = threadIdx.x / (D / 2), piece = threadIdx.x % (D / 2);
+    const bool carries = which < __popcll(runs);             // the same for the four lanes that exchange bytes
+    const uint8_t* run_from = nullptr;
+    if (carries) {
+        int in;
+        const uint8_t* const from = c.head(kv4_page(c, mine[kv4_run_start(runs, which)], in), 0);
+        run_from = from + kv4_value_tile<D>(c.P, in) + piece * 16;
     }
-    if (threadIdx.x < W / 16 * (D / 2)) {
-        const int which = threadIdx.x / (D / 2), j = threadIdx.x % (D / 2);
-        if (which < __popcll(runs)) {                        // the same for the four lanes that exchange bytes
-            int in;
-            const int pg = kv4_page(c, mine[kv4_run_start(runs, which)], in);
-            const u4 w = *reinterpret_cast<const u4*>(c.head(pg, h) + kv4_value_tile<D>(c.P, in) + j * 16);
-            const uint32_t quad_a = j & 1 ? 0x03070105u : 0x06020400u, quad_b = j & 2 ? 0x03020706u : 0x05040100u;
+    const uint32_t quad_a = piece & 1 ? 0x03070105u : 0x06020400u, quad_b = piece & 2 ? 0x03020706u : 0x05040100u;
+    const int shift = l >= LT / 2 ? 4 : 0;
+
+    for (int h = blockIdx.y; h < c.H; h += gridDim.y) {
+        const uint8_t* const head = page + (uint32_t)h * c.head_bytes;
+        u2 w[2] = {{0, 0}, {0, 0}};
+        uint32_t s[2] = {0, 0}, z[2] = {0, 0};
+        if (live) {
+            w[0] = *reinterpret_cast<const u2*>(head + kv4_key_row<D>(at) + byte);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {                    // bytes of four tokens -> this lane's token's byte of four lanes
-                uint32_t d = w[i];
-                d = __builtin_amdgcn_perm((uint32_t)dpp<kXor1>((int)d), d, quad_a);
-                d = __builtin_amdgcn_perm((uint32_t)dpp<kXor2>((int)d), d, quad_b);
-                *reinterpret_cast<uint32_t*>(rows + (which * 16 + 4 * i + kv4_place(j & 3)) * PITCH + (j & ~3)) = d;
+            for (int i = 0; i < 2; ++i) {
+                s[i] = *reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, i ? kValueScale : kKeyScale, g, at));
+                z[i] = *reinterpret_cast<const uint16_t*>(head + kv4_side<D, G>(c.P, i ? kValueZero : kKeyZero, g, at));
+            }
+            if (run < 0) {
+                const uint8_t* from = head + kv4_value_tile<D>(c.P, at) + kv4_place(at & 15) + byte * 16;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) w[1][j >> 2] |= (uint32_t)from[16 * j] << (8 * (j & 3));
             }
         }
-    }
-    __syncthreads();
-    if (t >= here) return;
-    if (run >= 0) w[1] = *reinterpret_cast<const u2*>(rows + (run * 16 + t - start) * PITCH + byte);
-    const int shift = l >= LT / 2 ? 4 : 0;
+        if (carries) {
+            const u4 x = *reinterpret_cast<const u4*>(run_from + (uint32_t)h * c.head_bytes);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        u4 out;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t u = w[i][j >> 1] >> (shift + 16 * (j & 1));
-            float x0 = ((float)(u & 15u) - z[i]) * s[i], x1 = ((float)((u >> 8) & 15u) - z[i]) * s[i];
-            // the products, then their rounding: fused into one mixed FMA with +0, -0 would become +0
-            asm("" : "+v"(x0), "+v"(x1));
-            out[j] = (uint32_t)store16(x0, bf16) | ((uint32_t)store16(x1, bf16) << 16);
+            for (int i = 0; i < 4; ++i) {                    // bytes of four tokens -> this lane's token's byte of four lanes
+                uint32_t d = x[i];
+                d = __builtin_amdgcn_perm((uint32_t)dpp<kXor1>((int)d), d, quad_a);
+                d = __builtin_amdgcn_perm((uint32_t)dpp<kXor2>((int)d), d, quad_b);
+                *reinterpret_cast<uint32_t*>(rows + (which * 16 + 4 * i + kv4_place(piece & 3)) * PITCH + (piece & ~3)) = d;
+            }
         }
-        *reinterpret_cast<u4*>((i ? v : k) + ((first + t) * c.H + h) * D + 8 * l) = out;
+        __syncthreads();
+        if (run >= 0) w[1] = *reinterpret_cast<const u2*>(rows + (run * 16 + t - start) * PITCH + byte);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const h2 sixteenth = {(_Float16)0.0625f, (_Float16)0.0625f}, base = {(_Float16)-64.f, (_Float16)-64.f};
+            const h2 less = base - __builtin_bit_cast(h2, z[i] * 0x10001u), scale = __builtin_bit_cast(h2, s[i] * 0x10001u);
+            u4 out;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {                    // bytes 0 1 and 2 3 to where one mask takes two
+                const uint32_t u = __builtin_amdgcn_perm(0, w[i][j >> 1] >> shift, j & 1 ? 0x0c030c02u : 0x0c010c00u);
+                const h2 code = __builtin_elementwise_fma(__builtin_bit_cast(h2, ((u << 4) & 0x00F000F0u) | 0x64006400u), sixteenth, less);
+                if constexpr (!BF16) {
+                    out[j] = __builtin_bit_cast(uint32_t, code * scale);
+                } else {
+                    out[j] = (uint32_t)store16((float)code[0] * (float)scale[0], 1) | ((uint32_t)store16((float)code[1] * (float)scale[1], 1) << 16);
+                }
+            }
+            if (t < here) *reinterpret_cast<u4*>((i ? v : k) + ((first + t) * c.H + h) * D + 8 * l) = live ? out : u4{0, 0, 0, 0};
+        }
+        __syncthreads();
     }
 }
 
@@ -257,12 +280,19 @@ int kv4_fail(int code, const char* who, const char* what) {
     return code;
 }
 
-// Calls f with the cache's sizes and the window: 64 tokens where that still gives every CU a workgroup, else 16.
+// Calls f with the cache's sizes, the window, the type and the grid.  Windows of 64 tokens catch most of a run that does
+// not start on a multiple of 16, and take fewer instructions a token; windows of 16 are more workgroups.  8192 tokens of
+// 8 heads at odd offsets written and read back 34.7 us in windows of 16, 31.4 in 64; 32768 tokens read 41.4 and 37.0.  A
+// workgroup takes as many heads of its window as still leaves kWindowGroups workgroups.
+constexpr int64_t kWindowGroups = 1024;
 template <class F>
-static void kv4_windows(const w4a16_kv4_cache* c, int64_t tokens, F f) {
+static void kv4_windows(const w4a16_kv4_cache* c, int64_t tokens, bool bf16, F f) {
     kv4_sizes(c, [&](auto d, auto g) {
         auto with = [&](auto w) {
-            f(d, g, w, dim3((unsigned)((tokens + w.value - 1) / w.value), (unsigned)c->kv_heads), dim3(w.value * d.value / 8));
+            const int64_t windows = (tokens + w.value - 1) / w.value;
+            const dim3 grid((unsigned)windows, (unsigned)std::min(c->kv_heads, std::max((int64_t)1, kWindowGroups / windows)));
+            if (bf16) f(d, g, w, std::true_type{}, grid, dim3(w.value * d.value / 8));
+            else f(d, g, w, std::false_type{}, grid, dim3(w.value * d.value / 8));
         };
         if (tokens * c->kv_heads >= 256 * 64) with(std::integral_constant<int, 64>{});
         else with(std::integral_constant<int, 16>{});
@@ -291,9 +321,9 @@ extern "C" int w4a16_kv4_write(const w4a16_kv4_cache* cache, const void* k, cons
         return kv4_fail(W4A16_ERR_INVALID, "kv4_write", "k and v must be 2-byte aligned, slots 8-byte aligned");
     const bool wide = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 && k_token_stride % 8 == 0 &&
                       k_head_stride % 8 == 0 && v_token_stride % 8 == 0 && v_head_stride % 8 == 0;
-    kv4_windows(cache, tokens, [&](auto d, auto g, auto w, dim3 grid, dim3 block) {
-        hipLaunchKernelGGL((kv4_write_kernel<d.value, g.value, w.value>), grid, block, 0, (hipStream_t)stream, kv4_of(cache),
-                           (const uint16_t*)k, (const uint16_t*)v, bf16, wide, (int)tokens, k_token_stride, k_head_stride, v_token_stride,
+    kv4_windows(cache, tokens, bf16, [&](auto d, auto g, auto w, auto b, dim3 grid, dim3 block) {
+        hipLaunchKernelGGL((kv4_write_kernel<d.value, g.value, w.value, b.value>), grid, block, 0, (hipStream_t)stream, kv4_of(cache),
+                           (const uint16_t*)k, (const uint16_t*)v, wide, (int)tokens, k_token_stride, k_head_stride, v_token_stride,
                            v_head_stride, slots);
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_write", hipGetErrorString(e));
@@ -309,9 +339,9 @@ extern "C" int w4a16_kv4_read(const w4a16_kv4_cache* cache, const int64_t* slots
     if (!k || !v || !slots) return kv4_fail(W4A16_ERR_INVALID, "kv4_read", "null pointer");
     if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 != 0 || reinterpret_cast<uintptr_t>(slots) % 8 != 0)
         return kv4_fail(W4A16_ERR_INVALID, "kv4_read", "k and v must be 16-byte aligned, slots 8-byte aligned");
-    kv4_windows(cache, tokens, [&](auto d, auto g, auto w, dim3 grid, dim3 block) {
-        hipLaunchKernelGGL((kv4_read_kernel<d.value, g.value, w.value>), grid, block, 0, (hipStream_t)stream, kv4_of(cache), slots,
-                           (int)tokens, bf16, (uint16_t*)k, (uint16_t*)v);
+    kv4_windows(cache, tokens, bf16, [&](auto d, auto g, auto w, auto b, dim3 grid, dim3 block) {
+        hipLaunchKernelGGL((kv4_read_kernel<d.value, g.value, w.value, b.value>), grid, block, 0, (hipStream_t)stream, kv4_of(cache), slots,
+                           (int)tokens, (uint16_t*)k, (uint16_t*)v);
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_read", hipGetErrorString(e));
     return W4A16_OK;
