@@ -142,7 +142,7 @@ def lib():
     L.w4a16_kv4_write.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_int] + [ctypes.c_int64] * 5 + [ctypes.c_void_p] * 2
     L.w4a16_kv4_read.argtypes = [ctypes.c_void_p] * 2 + [ctypes.c_int64, ctypes.c_int] + [ctypes.c_void_p] * 3
     L.w4a16_kv4_attention_workspace.argtypes = [ctypes.c_void_p] * 3
-    L.w4a16_kv4_attention.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int64, ctypes.c_void_p]
+    L.w4a16_kv4_attention.argtypes = [ctypes.c_void_p] * 4 + [ctypes.c_int64] + [ctypes.c_void_p] * 2
     return L
 
 
@@ -161,7 +161,7 @@ def test_c_entry_points_refuse_before_any_device_work(lib):
         assert word in lib.w4a16_last_error() and lib.w4a16_last_error().startswith(b"kv4_write")
         assert lib.w4a16_kv4_read(ctypes.byref(c), p, 1, 0, p, p, None) == 1 and word in lib.w4a16_last_error()
         assert lib.w4a16_kv4_attention_workspace(ctypes.byref(c), ctypes.byref(a), lim) == -1 and word in lib.w4a16_last_error()
-        assert lib.w4a16_kv4_attention(ctypes.byref(c), ctypes.byref(a), lim, None, 0, None) == 1 and word in lib.w4a16_last_error()
+        assert lib.w4a16_kv4_attention(ctypes.byref(c), ctypes.byref(a), lim, None, 0, p, None) == 1 and word in lib.w4a16_last_error()
     c = Cache(**ok)
     assert lib.w4a16_kv4_write(ctypes.byref(c), None, p, 0, 1, 256, 128, 256, 128, p, None) == 1 and b"null" in lib.w4a16_last_error()
     assert lib.w4a16_kv4_write(ctypes.byref(c), p + 1, p, 0, 1, 256, 128, 256, 128, p, None) == 1 and b"aligned" in lib.w4a16_last_error()
@@ -177,7 +177,7 @@ def test_c_entry_points_refuse_before_any_device_work(lib):
                          (dict(seq_lens=None), b"null"), (dict(block_table=None), b"null"), (dict(out=p + 4), b"aligned"), (dict(lse=p + 2), b"aligned"),
                          (dict(batch=2, tokens=2, table_stride=0), b"overlap"), (dict(table_width=1 << 27), b"range")]:
         a = Args(**{**good, **change})
-        assert lib.w4a16_kv4_attention(ctypes.byref(c), ctypes.byref(a), lim, None, 0, None) == 1, change
+        assert lib.w4a16_kv4_attention(ctypes.byref(c), ctypes.byref(a), lim, None, 0, p, None) == 1, change
         assert word in lib.w4a16_last_error(), (change, lib.w4a16_last_error())
 
 

@@ -32,6 +32,14 @@ typedef int i4v __attribute__((ext_vector_type(4)));
         v = op(v, dpp<kMirror>(v));        \
     } while (0)
 __device__ __forceinline__ float add(float a, float b) { return a + b; }
+__device__ __forceinline__ int add(int a, int b) { return a + b; }
+// Over the wave, as a scalar.
+template <class F>
+__device__ __forceinline__ int over_wave(int v, F f) {
+    W4A16_OVER_ROW(v, f);
+    return f(f(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
+}
 
 __device__ __forceinline__ void wave_lds_order() {           // a wave's own LDS operations stay in order
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -48,136 +56,72 @@ __device__ __forceinline__ float of_digits4(int d0, int d1, int d2, int d3) {
     return fmaf((float)((d3 << 8) + d2), 65536.f, (float)((d1 << 8) + d0));
 }
 
-// One workgroup takes one KV head of one sequence and a share of its tiles of 64 keys, a wave one tile at a time;
-// 4 NT rows (query, query head) at once.  Both products run on v_mfma_i32_16x16x64_i8: the codes are its operand as
-// they lie in the cache (one mask, for the upper codes one shift), the other operand is a fixed-point number in
-// digits, which fill the rows that four query heads leave of the 16: row 4 r + i is digit i of row r.
+// Partial results are written and read at agent scope: workgroups of other XCDs, with L2 caches of their own, join them.
+__device__ __forceinline__ void put_shared(float* p, float a, float b) {
+    const uint64_t v = (uint64_t)__builtin_bit_cast(uint32_t, a) | ((uint64_t)__builtin_bit_cast(uint32_t, b) << 32);
+    __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 get_shared(const float* p) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const uint32_t lo = (uint32_t)v, hi = (uint32_t)(v >> 32);
+    return float2{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
+}
+
+// A workgroup takes one KV head of one sequence and a share of its tiles of 64 keys, its waves a tile each in turn; 4 NT rows
+// (query, query head) at once.  The last of a head's workgroups to finish joins their results.
+//
+// Both products run on v_mfma_i32_16x16x64_i8: the codes are its operand as they lie in the cache (a shift and a mask), the
+// other operand is a fixed-point number in digits, which fill the rows that four query heads leave of the 16: row 4 r + i
+// is digit i of row r.
 //   scores  x = rs s_t (sum_d q_d c_td - z_t sum_d q_d)     q to 2^-22 of the power of two above its row's largest
 //   values  o = sum_t (p_t s_t) (8 c_td - 8 z_t) / 8         p s to 2^-30 of the power of two above the tile's largest s
 // The integer sums are exact, those of 8 z_t (in two digits, one more column of the product) among them, and are taken
-// off digit by digit: a value that is 0 weighs nothing however large p is.  The digits come together in fp32.  Per 64 keys a wave issues about 300 vector
-// instructions for 8.7 KB, under a third of the time that HBM takes to bring them.
+// off digit by digit: a value that is 0 weighs nothing however large p is.  The digits come together in fp32.
+//
+// ONE: the page size is a multiple of 64, so a tile lies in one page and its addresses are the wave's.
 template <int D, int G, int NT, int WAVES, bool ONE>
-__global__ void __launch_bounds__(64 * WAVES)
-kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
-                 float* __restrict__ part_o) {
-    constexpr int NG = D / G;                                // groups of a token: of lower and of upper codes where 2
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 && D == G && WAVES == 4 ? 3 : NT <= 2 ? 2 : 1)))
+kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
+    constexpr int NG = D / G, ROWS = 4 * NT, THREADS = 64 * WAVES;      // NG 2: groups of lower and of upper codes
     constexpr int NV = D / 32;                               // 16-byte pieces per lane of a value tile
     constexpr int kSide = NG * (64 * 8 + 128), kDigits = NT * NG * 1024;
-    constexpr int kLoop = WAVES * (kSide + kDigits), kJoin = WAVES * 4 * NT * (D + 2) * 4;
+    constexpr int kLoop = WAVES * (kSide + kDigits), kJoin = WAVES * ROWS * (D + 2) * 4;
     __shared__ __align__(16) uint8_t lds[kLoop > kJoin ? kLoop : kJoin];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ __align__(16) uint8_t q_digits[ROWS * 4 * D];
+    __shared__ float q_scale[ROWS], q_sum[ROWS][NG];
+    __shared__ int last_one;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     uint8_t* const side = lds + wave * (kSide + kDigits);
     uint8_t* const dig = side + kSide;
+    const int units = ONE ? a.c.P >> 6 : a.c.P >> 4;         // tiles, or groups of 16 tokens, of a page
     const int h = blockIdx.x % a.c.H, split = blockIdx.x / a.c.H, b = blockIdx.y;
     const Kv4Seq s = kv4_seq(a, b);
     const int rows = s.count * a.rep, base = s.len - s.count;
-    const int units = ONE ? a.c.P >> 6 : a.c.P >> 4;         // tiles, or groups of 16 tokens, of a page
     const int* const table = a.table + b * a.table_stride;
-    const uint8_t* const mine = a.c.data + (uint64_t)(uint32_t)h * a.c.head_bytes;      // this head's bytes of page 0
+    const uint8_t* const mine = a.c.data + (uint64_t)(uint32_t)h * a.c.head_bytes;          // this head's bytes of page 0
 
-    for (int row0 = 0; row0 < rows; row0 += 4 * NT) {
-        int lane = threadIdx.x & 63;
-        asm volatile("" : "+v"(lane));                       // what follows from it is not kept in registers across passes
-        const int kb = lane >> 4, n = lane & 15;
-        const uint32_t quad_a = lane & 1 ? 0x03070105u : 0x06020400u;   // selectors of the 4 x 4 byte transpose below
-        const uint32_t quad_b = lane & 2 ? 0x03070206u : 0x05010400u;
-        const int first = row0 / a.rep, last = (min(row0 + 4 * NT, rows) - 1) / a.rep;
+    for (int row0 = 0; row0 < rows; row0 += ROWS) {
+        const int first = row0 / a.rep, last = (min(row0 + ROWS, rows) - 1) / a.rep;
         const int kmax = a.causal ? max(0, min(base + last + 1, s.len)) : s.len;
         const int kmin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
         const int tile0 = kmin >> 6, tiles = a.c.pages > 0 ? max(0, ((kmax + 63) >> 6) - tile0) : 0;
-        const int per = max(WAVES, (tiles + splits - 1) / splits), parts = max(1, (tiles + per - 1) / per);
-        if (split >= parts) continue;
+        // more rows than one pass takes (max_q was too small for them) are not shared out
+        const int per = rows > ROWS ? max(tiles, 1) : max(WAVES, (tiles + splits - 1) / splits), parts = max(1, (tiles + per - 1) / per);
+        if (split >= parts) return;
+        int lane = tid & 63;
+        asm volatile("" : "+v"(lane));                       // what follows from it is not kept in registers across passes
+        const int kb = lane >> 4, n = lane & 15;
         // keys that every row sees: no masks where a tile lies within
         const int sure_end = a.causal ? min(base + first + 1, s.len) : s.len;
         const int sure_begin = a.window > 0 ? max(0, base + last - a.window + 1) : 0;
-
-        // The rows' queries as digits, in the order of the cache's bytes
-        i4v qd[NT][D / 64];
-        float rs[NT], qsum[NT][NG];
-        int begin[NT], end[NT];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const int r = row0 + 4 * t + (n >> 2);
-            float x[D / 64][16];
-            uint32_t top = 0;
-            if (r < rows) {
-                const uint16_t* src = a.q + (int64_t)(s.first + r / a.rep) * a.q_token + (int64_t)(h * a.rep + r % a.rep) * a.q_head + 16 * kb;
-#pragma unroll
-                for (int i = 0; i < D / 64; ++i) {
-                    if (a.q_wide) {
-                        const u4 lo = *reinterpret_cast<const u4*>(src + 64 * i), hi = *reinterpret_cast<const u4*>(src + 64 * i + 8);
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const uint32_t w0 = lo[j], w1 = hi[j];
-                            x[i][2 * j] = load16(w0 & 0xFFFF, a.bf16);
-                            x[i][2 * j + 1] = load16(w0 >> 16, a.bf16);
-                            x[i][8 + 2 * j] = load16(w1 & 0xFFFF, a.bf16);
-                            x[i][8 + 2 * j + 1] = load16(w1 >> 16, a.bf16);
-                        }
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) x[i][j] = load16(src[64 * i + j], a.bf16);
-                    }
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) x[i][j] = 0.f;
-            }
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i)
-#pragma unroll
-                for (int j = 0; j < 16; ++j) top = max(top, __builtin_bit_cast(uint32_t, x[i][j]) & 0x7FFFFFFFu);
-            top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-            top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-            const bool finite = top < 0x7F800000u;
-            const int e = finite ? __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) : 0;   // |x| < 2^e
-            int sums[D / 64];
-#pragma unroll
-            for (int i = 0; i < D / 64; ++i) {
-                int sum = 0;
-                uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int v = finite ? (int)rintf(ldexpf(x[i][j], 22 - e)) : 0;
-                    sum += v;
-                    w[j >> 2] |= ((digits3(v) >> (8 * (n & 3))) & 0xFFu) << (8 * (j & 3));
-                }
-                qd[t][i] = i4v{(int)w[0], (int)w[1], (int)w[2], (int)w[3]};
-                sum += __shfl_xor(sum, 16, 64);
-                sums[i] = sum + __shfl_xor(sum, 32, 64);
-            }
-            // from here on lane (kb, n) stands for row kb
-#pragma unroll
-            for (int g = 0; g < NG; ++g) {
-                const int sum = NG == 2 || D == 64 ? sums[g] : sums[0] + sums[D / 64 - 1];
-                qsum[t][g] = (float)__shfl(sum, 4 * kb, 64);
-            }
-            rs[t] = __shfl(finite ? fmaxf(ldexpf(a.scale2, e - 22), 0x1p-126f) : NAN, 4 * kb, 64);
-            const int own = row0 + 4 * t + kb, pos = base + own / a.rep;
-            end[t] = own < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
-            begin[t] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-        }
-
-        float m[NT], l[NT], nan[NT][NG], o[NT][2][NV];
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            m[t] = -INFINITY;
-            l[t] = 0.f;
-#pragma unroll
-            for (int g = 0; g < NG; ++g) nan[t][g] = 0.f;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) o[t][0][i] = o[t][1][i] = 0.f;
-        }
+        const uint32_t quad_a = lane & 1 ? 0x03070105u : 0x06020400u;   // selectors of the 4 x 4 byte transpose below
+        const uint32_t quad_b = lane & 2 ? 0x03070206u : 0x05010400u;
 
         // What a lane holds of a tile of 64 tokens.  Each part of the next tile is sent for where this tile's has been used.
         u4 k[4];                                             // 16 bytes of the row of token 16 r + n
         u4 v[NV];                                            // tokens 16 kb .. + 15 of byte n + 16 i
         uint16_t sides[4][NG];                               // of token 16 kb + n
-        // Where they come from: the page's bytes of this head and the place in it of the tile (ONE: every tile lies in one
-        // page, so for the whole wave) or of tokens 16 kb .. + 15 (for the lane)
+        // Where they come from: the page's bytes of this head and the place in it of the tile (ONE) or of tokens 16 kb .. + 15
         bool there = false;                                  // the page is in the cache
         uint64_t kv = 0;
         int place = 0;
@@ -185,7 +129,7 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             const int unit = ONE ? tile : tile * 4 + kb;
             return units == 1 ? unit : (int)__umulhi((uint32_t)unit, page_magic);
         };
-        auto entry = [&](int tile) { return ONE || tile * 64 + kb * 16 < kmax ? table[entry_at(tile)] : -1; };
+        auto entry = [&](int tile) { return tile * 64 + (ONE ? 0 : kb * 16) < kmax ? table[entry_at(tile)] : -1; };
         auto aim = [&](int tile, int page) {
             place = ONE ? (tile - entry_at(tile) * units) * 64 : (tile * 4 + kb - entry_at(tile) * units) * 16;
             there = (uint32_t)page < (uint32_t)a.c.pages;
@@ -203,19 +147,19 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             const uint64_t at = kv + kv4_key_row<D>(place);
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const uint32_t in = n * (D / 2) + 16 * (D == 128 ? kb : kb & 1);
+                const uint32_t off = n * (D / 2) + 16 * (D == 128 ? kb : kb & 1);
                 uint64_t row = at + r * 16 * (D / 2);
                 if constexpr (!ONE)
                     row = ((uint64_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), 16 * r) << 32) |
                           __builtin_amdgcn_readlane((uint32_t)at, 16 * r);
-                k[r] = *reinterpret_cast<const u4*>(mine + row + in);
+                k[r] = *reinterpret_cast<const u4*>(mine + row + off);
             }
         };
         auto load_values = [&] {
             const uint8_t* vals = mine + kv + kv4_value_tile<D>(a.c.P, place);
-            const uint32_t in = n * 16 + (ONE ? kb * (D / 2 * 16) : 0);
+            const uint32_t off = n * 16 + (ONE ? kb * (D / 2 * 16) : 0);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const u4*>(vals + in + 256 * i);
+            for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const u4*>(vals + off + 256 * i);
         };
 
         const int stop = tile0 + min(tiles, (split + 1) * per);
@@ -227,6 +171,63 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             load_values();
             if (tile + WAVES < stop) page = entry(tile + WAVES);
         }
+
+        // The rows' queries as digits, a wave to a row, while the first tile is on its way
+        for (int r = wave; r < ROWS; r += WAVES) {
+            const int row = row0 + r;
+            float x[D / 64];
+            uint32_t top = 0;
+            const uint16_t* src = a.q + (int64_t)(s.first + row / a.rep) * a.q_token + (int64_t)(h * a.rep + row % a.rep) * a.q_head;
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                x[i] = row < rows ? load16(src[lane + 64 * i], a.bf16) : 0.f;
+                top = max(top, __builtin_bit_cast(uint32_t, x[i]) & 0x7FFFFFFFu);
+            }
+            top = (uint32_t)over_wave((int)top, [](int p, int q) { return max(p, q); });
+            const bool finite = top < 0x7F800000u;
+            const int e = finite ? __builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, top)) : 0;   // |x| < 2^e
+            int sums[D / 64];
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) {
+                const int y = finite ? (int)rintf(ldexpf(x[i], 22 - e)) : 0;
+                const uint32_t w = digits3(y);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) q_digits[(r * 4 + j) * D + lane + 64 * i] = (uint8_t)(w >> (8 * j));
+                sums[i] = over_wave(y, [](int p, int q) { return p + q; });
+            }
+            if (lane == 0) {
+                q_scale[r] = finite ? fmaxf(ldexpf(a.scale2, e - 22), 0x1p-126f) : NAN;
+#pragma unroll
+                for (int g = 0; g < NG; ++g) q_sum[r][g] = (float)(NG == 2 || D == 64 ? sums[g] : sums[0] + sums[D / 64 - 1]);
+            }
+        }
+        __syncthreads();
+        i4v qd[NT][D / 64];
+        float rs[NT], qsum[NT][NG];
+        int begin[NT], end[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+#pragma unroll
+            for (int i = 0; i < D / 64; ++i) qd[t][i] = *reinterpret_cast<const i4v*>(q_digits + (16 * t + n) * D + 64 * i + 16 * kb);
+            rs[t] = q_scale[4 * t + kb];
+#pragma unroll
+            for (int g = 0; g < NG; ++g) qsum[t][g] = q_sum[4 * t + kb][g];
+            const int own = row0 + 4 * t + kb, pos = base + own / a.rep;
+            end[t] = own < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
+            begin[t] = a.window > 0 ? max(0, pos - a.window + 1) : 0;
+        }
+
+        float m[NT], l[NT], nan[NT][NG], o[NT][2][NV];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            m[t] = -INFINITY;
+            l[t] = 0.f;
+#pragma unroll
+            for (int g = 0; g < NG; ++g) nan[t][g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) o[t][0][i] = o[t][1][i] = 0.f;
+        }
+
         for (; tile < stop; tile += WAVES) {
             const bool more = tile + WAVES < stop, here = there;
             // scales and zeros through LDS, nothing for tokens that no row sees; the largest value scale
@@ -383,8 +384,8 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
 
         // The waves' shares come together in LDS
         float* const jm = reinterpret_cast<float*>(lds);
-        float* const jl = jm + WAVES * 4 * NT;
-        float* const jo = jl + WAVES * 4 * NT;
+        float* const jl = jm + WAVES * ROWS;
+        float* const jo = jl + WAVES * ROWS;
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -392,7 +393,7 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             W4A16_OVER_ROW(sum, add);
 #pragma unroll
             for (int g = 0; g < NG; ++g) W4A16_OVER_ROW(nan[t][g], add);
-            const int r = wave * 4 * NT + 4 * t + kb;
+            const int r = wave * ROWS + 4 * t + kb;
             if (n == 0) {
                 jm[r] = m[t];
                 jl[r] = sum;
@@ -404,71 +405,107 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, int* __restrict__ u
             }
         }
         __syncthreads();
-        for (int i = threadIdx.x; i < 4 * NT * (D / 2); i += 64 * WAVES) {
-            const int r = i / (D / 2), d = i % (D / 2) * 2, own = row0 + r;
-            if (own >= rows) continue;
+        auto row_at = [&](int r) { return (int64_t)(s.first + r / a.rep) * a.heads + h * a.rep + r % a.rep; };
+        const int64_t item = (int64_t)b * a.c.H + h, slot = item * splits + split;
+        for (int i = tid; i < ROWS * (D / 2); i += THREADS) {
+            const int r = i / (D / 2), d = i % (D / 2) * 2;
             float top = jm[r];
 #pragma unroll
-            for (int w = 1; w < WAVES; ++w) top = fmaxf(top, jm[w * 4 * NT + r]);
+            for (int w = 1; w < WAVES; ++w) top = fmaxf(top, jm[w * ROWS + r]);
             const float safe = top == -INFINITY ? 0.f : top;
             float sum = 0.f, v0 = 0.f, v1 = 0.f;
 #pragma unroll
             for (int w = 0; w < WAVES; ++w) {
-                const float f = __builtin_amdgcn_exp2f(jm[w * 4 * NT + r] - safe);
-                const float2 y = *reinterpret_cast<const float2*>(jo + (w * 4 * NT + r) * D + d);
-                sum = fmaf(f, jl[w * 4 * NT + r], sum);
+                const float f = __builtin_amdgcn_exp2f(jm[w * ROWS + r] - safe);
+                const float2 y = *reinterpret_cast<const float2*>(jo + (w * ROWS + r) * D + d);
+                sum = fmaf(f, jl[w * ROWS + r], sum);
                 v0 = fmaf(f, y.x, v0);
                 v1 = fmaf(f, y.y, v1);
             }
-            const int64_t row = (int64_t)(s.first + own / a.rep) * a.heads + h * a.rep + own % a.rep;
             if (parts == 1) {
-                kv4_finish<D>(a, row, d, top, sum, v0, v1);
-                if (used && d == 0) used[row] = 1;
+                if (row0 + r < rows) kv4_finish<D>(a, row_at(row0 + r), d, top, sum, v0, v1);
             } else {
-                const int64_t at = row * splits + split;
-                *reinterpret_cast<float2*>(part_o + at * D + d) = float2{v0, v1};
-                if (d == 0) {
-                    part_ml[at] = float2{top, sum};
-                    if (split == 0) used[row] = parts;
-                }
+                put_shared(parts_o + (slot * ROWS + r) * D + d, v0, v1);
+                if (d == 0) put_shared(parts_ml + (slot * ROWS + r) * 2, top, sum);
             }
         }
-        __syncthreads();
+        if (parts > 1) {                                     // one pass only: rows <= ROWS
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (tid == 0) {
+                last_one = __hip_atomic_fetch_add(counters + item, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+                if (last_one) __hip_atomic_store(counters + item, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+            __syncthreads();
+            if (!last_one) return;
+            // Four values a thread; sets of threads take the parts in turn and come together in LDS, always in one order.
+            constexpr int Q = ROWS * D / 4, SETS = THREADS / Q > 1 ? THREADS / Q : 1, BATCH = 8;
+            const int set = SETS > 1 ? tid / Q : 0;
+            float* const js = reinterpret_cast<float*>(lds);             // [SETS][Q][6]
+            for (int i = SETS > 1 ? tid % Q : tid; i < Q; i += SETS > 1 ? Q : THREADS) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int p0 = set; p0 < parts; p0 += SETS * BATCH) {
+                    float2 ml[BATCH], x[BATCH], y[BATCH];
+#pragma unroll
+                    for (int p = 0; p < BATCH; ++p) {
+                        const int64_t from = (item * splits + min(p0 + p * SETS, parts - 1)) * ROWS + r;
+                        ml[p] = get_shared(parts_ml + from * 2);
+                        x[p] = get_shared(parts_o + from * D + d);
+                        y[p] = get_shared(parts_o + from * D + d + 2);
+                    }
+                    float next = top;
+#pragma unroll
+                    for (int p = 0; p < BATCH; ++p)
+                        if (p0 + p * SETS < parts) next = fmaxf(next, ml[p].x);
+                    const float safe = next == -INFINITY ? 0.f : next, keep = __builtin_amdgcn_exp2f(top - safe);
+                    top = next;
+                    sum *= keep;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[j] *= keep;
+#pragma unroll
+                    for (int p = 0; p < BATCH; ++p) {
+                        const bool real = p0 + p * SETS < parts;
+                        const float f = real ? __builtin_amdgcn_exp2f(ml[p].x - safe) : 0.f;
+                        sum = fmaf(f, real ? ml[p].y : 0.f, sum);
+                        v[0] = fmaf(f, real ? x[p].x : 0.f, v[0]);
+                        v[1] = fmaf(f, real ? x[p].y : 0.f, v[1]);
+                        v[2] = fmaf(f, real ? y[p].x : 0.f, v[2]);
+                        v[3] = fmaf(f, real ? y[p].y : 0.f, v[3]);
+                    }
+                }
+                if constexpr (SETS > 1) {
+                    float* const to = js + (set * Q + i) * 6;
+                    to[0] = top;
+                    to[1] = sum;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) to[2 + j] = v[j];
+                    __syncthreads();                         // one turn of the loop: every thread is here
+                    if (set > 0) return;
+                    float next = -INFINITY;
+#pragma unroll
+                    for (int w = 0; w < SETS; ++w) next = fmaxf(next, js[(w * Q + i) * 6]);
+                    const float safe = next == -INFINITY ? 0.f : next;
+                    top = next;
+                    sum = v[0] = v[1] = v[2] = v[3] = 0.f;
+#pragma unroll
+                    for (int w = 0; w < SETS; ++w) {
+                        const float* const from = js + (w * Q + i) * 6;
+                        const float f = __builtin_amdgcn_exp2f(from[0] - safe);
+                        sum = fmaf(f, from[1], sum);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = fmaf(f, from[2 + j], v[j]);
+                    }
+                }
+                if (row0 + r < rows) {
+                    kv4_finish<D>(a, row_at(row0 + r), d, top, sum, v[0], v[1]);
+                    kv4_finish<D>(a, row_at(row0 + r), d + 2, top, sum, v[2], v[3]);
+                }
+            }
+            return;
+        }
+        __syncthreads();                                     // before the next pass's queries and tiles go into LDS
     }
-}
-
-// Joins the shares of one row (used[row] of them, each of its own part of the keys): one workgroup per row.
-template <int D>
-__global__ void __launch_bounds__(256)
-kv4_join_kernel(Kv4Attn a, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml, const float* __restrict__ part_o) {
-    constexpr int Q = D / 4, R = 256 / Q;                    // threads of one share, shares at once
-    __shared__ float weight[256], sums[256];
-    __shared__ f4 acc[256];
-    const int64_t row = blockIdx.x;
-    const int parts = min(used[row], splits);
-    if (parts <= 1) return;
-    const int t = threadIdx.x;
-    const float2 ml = t < parts ? part_ml[row * splits + t] : float2{-INFINITY, 0.f};
-    weight[t] = ml.x;
-    __syncthreads();
-    float top = -INFINITY;
-    for (int i = 0; i < parts; ++i) top = fmaxf(top, weight[i]);
-    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
-    __syncthreads();
-    weight[t] = f;
-    sums[t] = f * ml.y;
-    __syncthreads();
-    float sum = 0.f;
-    for (int i = 0; i < parts; ++i) sum += sums[i];
-    f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = t / Q; i < parts; i += R) v += weight[i] * *reinterpret_cast<const f4*>(part_o + (row * splits + i) * D + t % Q * 4);
-    acc[t] = v;
-    __syncthreads();
-    if (t >= Q) return;
-    for (int i = 1; i < R; ++i) v += acc[i * Q + t];
-    kv4_finish<D>(a, row, 4 * t, top, sum, v[0], v[1]);
-    kv4_finish<D>(a, row, 4 * t + 2, top, sum, v[2], v[3]);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -842,6 +879,40 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
     }
 }
 
+// Joins the shares of one row (used[row] of them, each of its own part of the keys): one workgroup per row.
+template <int D>
+__global__ void __launch_bounds__(256)
+kv4_join_kernel(Kv4Attn a, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml, const float* __restrict__ part_o) {
+    constexpr int Q = D / 4, R = 256 / Q;                    // threads of one share, shares at once
+    __shared__ float weight[256], sums[256];
+    __shared__ f4 acc[256];
+    const int64_t row = blockIdx.x;
+    const int parts = min(used[row], splits);
+    if (parts <= 1) return;
+    const int t = threadIdx.x;
+    const float2 ml = t < parts ? part_ml[row * splits + t] : float2{-INFINITY, 0.f};
+    weight[t] = ml.x;
+    __syncthreads();
+    float top = -INFINITY;
+    for (int i = 0; i < parts; ++i) top = fmaxf(top, weight[i]);
+    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+    __syncthreads();
+    weight[t] = f;
+    sums[t] = f * ml.y;
+    __syncthreads();
+    float sum = 0.f;
+    for (int i = 0; i < parts; ++i) sum += sums[i];
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = t / Q; i < parts; i += R) v += weight[i] * *reinterpret_cast<const f4*>(part_o + (row * splits + i) * D + t % Q * 4);
+    acc[t] = v;
+    __syncthreads();
+    if (t >= Q) return;
+    for (int i = 1; i < R; ++i) v += acc[i * Q + t];
+    kv4_finish<D>(a, row, 4 * t, top, sum, v[0], v[1]);
+    kv4_finish<D>(a, row, 4 * t + 2, top, sum, v[2], v[3]);
+}
+
 static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_attention_args* a, const w4a16_device_limits* lim) {
     if (const char* m = kv4_check(c)) return m;
     if (!a || !lim) return "null pointer";
@@ -849,6 +920,8 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
         a->batch >= 65536 || a->table_width * c->page_size >= (int64_t)1 << 27 || a->max_q < 1 || a->window < 0 ||
         a->tokens * a->heads >= (int64_t)1 << 31 || a->batch * a->heads >= (int64_t)1 << 31)
         return "dimensions out of range";
+    if ((a->tokens * (a->heads / c->kv_heads) / 4 + a->batch) * c->kv_heads >= ((int64_t)1 << 31) / std::max<int64_t>(1, a->table_width * c->page_size / 64 + 1))
+        return "too many queries times keys";
     if (a->heads % c->kv_heads != 0) return "the query heads must be a multiple of the KV heads";
     if (!a->q_start && a->tokens != a->batch) return "without q_start there is one query per sequence";
     if (!(a->scale > 0.f) || !isfinite(a->scale)) return "scale must be positive and finite";
@@ -862,28 +935,33 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
     return nullptr;
 }
 
-// How a call runs: rows of one pass of the token kernel (4 nt; 0: the prompt kernel, row_tiles workgroups), shares of the keys of one row, and
-// the workspace: per row (query, query head) the number of shares, then (largest score, sum) and sums of each share.
+// How a call runs.  The token kernel (nt: its rows are 4 nt, in workgroups of `waves`) or the prompt kernel on row_tiles
+// workgroups a sequence and head; both times `splits` shares of the keys, whose results the workspace holds.
 constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
 struct AttnPlan {
-    int nt, splits, row_tiles;
+    int nt, waves, row_tiles, splits;
     int64_t ml_at, o_at, bytes;
 };
 
-static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attention_args& a) {
+static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attention_args& a, const w4a16_device_limits& lim) {
     AttnPlan p{};
-    const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep;
-    p.splits = 1;
+    const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep, items = a.batch * c.kv_heads;
     int64_t tiles = (a.table_width * c.page_size + 63) / 64;
     if (a.window > 0) tiles = std::min(tiles, (a.window + a.max_q) / 64 + 2);
-    int64_t wanted;
+    p.splits = 1;
     if (rows <= 16) {
         p.nt = rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
-        wanted = 2048 / (a.batch * c.kv_heads);
-    } else {
-        p.row_tiles = (int)std::min<int64_t>((rows + kPromptRows - 1) / kPromptRows, 65535);
-        wanted = 512 / (a.batch * c.kv_heads * p.row_tiles);
+        p.waves = p.nt <= 2 && items <= 64 && c.page_size % 64 == 0 ? 8 : 4;
+        const int64_t wanted = (p.waves == 8 ? 256 : 2048) / items;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + p.waves - 1) / p.waves, W4A16_KV4_COUNTERS / items}));
+        if (p.splits > 1) {
+            p.o_at = items * p.splits * 4 * p.nt * 8;
+            p.bytes = p.o_at + items * p.splits * 4 * p.nt * c.head_dim * 4;
+        }
+        return p;
     }
+    p.row_tiles = (int)std::min<int64_t>((rows + kPromptRows - 1) / kPromptRows, 65535);
+    const int64_t wanted = 512 / (a.batch * c.kv_heads * p.row_tiles);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + 3) / 4, 256}));
     if (p.splits > 1) {
         const int64_t all = a.tokens * a.heads;
@@ -901,15 +979,17 @@ using namespace w4a16;
 extern "C" int64_t w4a16_kv4_attention_workspace(const w4a16_kv4_cache* cache, const w4a16_kv4_attention_args* args,
                                                  const w4a16_device_limits* lim) {
     if (const char* m = check_attention(cache, args, lim)) return kv4_fail(-1, "kv4_attention", m);
-    return args->tokens == 0 || args->batch == 0 ? 0 : plan_attention(*cache, *args).bytes;
+    return args->tokens == 0 || args->batch == 0 ? 0 : plan_attention(*cache, *args, *lim).bytes;
 }
 
 extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4_attention_args* args, const w4a16_device_limits* lim,
-                                   void* workspace, int64_t workspace_bytes, void* stream) {
+                                   void* workspace, int64_t workspace_bytes, int32_t* counters, void* stream) {
     const int64_t need = w4a16_kv4_attention_workspace(cache, args, lim);
     if (need < 0) return W4A16_ERR_INVALID;
     if (workspace_bytes < need || (need && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 != 0)))
         return kv4_fail(W4A16_ERR_WORKSPACE, "kv4_attention", "workspace missing, unaligned or too small");
+    if (!counters || reinterpret_cast<uintptr_t>(counters) % 4 != 0)
+        return kv4_fail(W4A16_ERR_WORKSPACE, "kv4_attention", "counters missing or unaligned");
     if (args->tokens == 0 || args->batch == 0) return W4A16_OK;
     Kv4Attn a{};
     a.c = kv4_of(cache);
@@ -931,7 +1011,7 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
     a.bf16 = args->bf16 != 0;
     a.causal = args->causal != 0;
     a.q_wide = reinterpret_cast<uintptr_t>(args->q) % 16 == 0 && args->q_token_stride % 8 == 0 && args->q_head_stride % 8 == 0;
-    const AttnPlan plan = plan_attention(*cache, *args);
+    const AttnPlan plan = plan_attention(*cache, *args, *lim);
     const hipStream_t st = (hipStream_t)stream;
     char* const ws = (char*)workspace;
     int* const used = plan.splits > 1 ? (int*)ws : nullptr;
@@ -944,12 +1024,14 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
             const uint32_t magic = magic_of(cache->page_size / (one ? 64 : 16));
             const dim3 grid((unsigned)(cache->kv_heads * plan.splits), (unsigned)args->batch);
             auto launch = [&](auto nt) {
-                if (one)
-                    hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4, true>), grid, dim3(256), 0, st, a, plan.splits, magic,
-                                       used, ml, po);
-                else
-                    hipLaunchKernelGGL((kv4_token_kernel<d.value, g.value, nt.value, 4, false>), grid, dim3(256), 0, st, a, plan.splits, magic,
-                                       used, ml, po);
+                auto on = [&](auto kernel, int waves) {
+                    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, plan.splits, magic, (float*)ws, po, counters);
+                };
+                if constexpr (nt.value <= 2) {
+                    if (plan.waves == 8) return on(kv4_token_kernel<d.value, g.value, nt.value, 8, true>, 8);
+                }
+                if (one) on(kv4_token_kernel<d.value, g.value, nt.value, 4, true>, 4);
+                else on(kv4_token_kernel<d.value, g.value, nt.value, 4, false>, 4);
             };
             if (plan.nt == 1) launch(std::integral_constant<int, 1>{});
             else if (plan.nt == 2) launch(std::integral_constant<int, 2>{});
@@ -958,10 +1040,10 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
             const dim3 grid((unsigned)cache->kv_heads, (unsigned)(plan.row_tiles * plan.splits), (unsigned)args->batch);
             hipLaunchKernelGGL((kv4_prompt_kernel<d.value, g.value, kPromptWaves>), grid, dim3(64 * kPromptWaves), 0, st, a, plan.row_tiles,
                                plan.splits, magic_of(cache->page_size / 16), used, ml, po);
+            if (plan.splits > 1)
+                hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits,
+                                   used, ml, po);
         }
-        if (plan.splits > 1)
-            hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits, used,
-                               ml, po);
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_attention", hipGetErrorString(e));
     return W4A16_OK;

@@ -16,6 +16,7 @@
 #include <tuple>
 
 #include "w4a16.h"
+#include "w4a16_counters.h"
 
 namespace {
 
@@ -142,7 +143,10 @@ py::object kv4_attention(torch::Tensor q, torch::Tensor cache, torch::Tensor blo
     TORCH_CHECK(bytes >= 0, w4a16_last_error());
     torch::Tensor ws;
     if (bytes) ws = torch::empty({bytes}, q.options().dtype(torch::kUInt8));
-    const int rc = w4a16_kv4_attention(&c, &a, &lim, bytes ? ws.data_ptr() : nullptr, bytes, stream_of(q));
+    const hipStream_t stream = c10::hip::getCurrentHIPStream(q.device().index()).stream();
+    if (!pool_ready(q.device().index()) && !capturing(stream)) ensure_capture_pool(q);
+    const torch::Tensor counters = split_counters(q, stream, W4A16_KV4_COUNTERS, W4A16_KV4_COUNTERS);
+    const int rc = w4a16_kv4_attention(&c, &a, &lim, bytes ? ws.data_ptr() : nullptr, bytes, counters.data_ptr<int32_t>(), stream);
     TORCH_CHECK(rc == W4A16_OK, w4a16_last_error());
     return return_lse ? py::cast(std::make_tuple(out, lse)) : py::cast(out);
 }

@@ -13,111 +13,16 @@
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
 
-#include <atomic>
 #include <chrono>
 #include <initializer_list>
 #include <vector>
-#include <map>
-#include <mutex>
-
 #include <string>
 
 #include "w4a16.h"
+#include "w4a16_counters.h"
 #include "w4a16_internal.h"
 
 namespace {
-
-// Split-K counters (decode split-K and the long-K prefill token-group configs, which run one
-// K segment per workgroup).  Launches that share a counter buffer must not overlap in time
-// (w4a16.h), and work on different streams may overlap, so:
-//  * eager calls keep one buffer per (device, stream): zeroed when created, left zero by every
-//    launch;
-//  * a call made under HIP graph capture gets a slice of its own from a per-device pool that the
-//    first eager call on the device zeroed; a slice is never handed out again, so graph nodes and
-//    eager work never share counters, and every replay leaves its slice zero for the next one.
-//    A graph must not be replayed concurrently with itself (its nodes own their slices).
-//  * if the pool is missing (no eager call before the capture) or used up, the captured call
-//    allocates its counters from the capture's memory pool and zeroes them with a fill kernel
-//    that the graph records (correct, one extra graph node per such call).
-// The returned tensor must stay alive until the launch is enqueued.
-constexpr int64_t kCapturePoolSlots = 1 << 20;
-
-struct CapturePool {
-    at::Tensor buf;
-    int64_t next = 0;
-};
-
-std::mutex g_mu;
-std::map<std::pair<int, hipStream_t>, at::Tensor> g_counters;
-std::map<int, CapturePool> g_capture_pool;
-// Set once a device's pool exists (cleared by the test hook that drops it): lets every later
-// call skip the capture-status query that guards the pool's creation (~0.16 us per call).
-constexpr int kMaxPoolDevices = 64;
-std::atomic<bool> g_pool_ready[kMaxPoolDevices];
-
-bool pool_ready(int dev) {
-    return dev >= 0 && dev < kMaxPoolDevices && g_pool_ready[dev].load(std::memory_order_acquire);
-}
-
-bool capturing(hipStream_t stream) {
-    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    TORCH_CHECK(hipStreamIsCapturing(stream, &st) == hipSuccess, "hipStreamIsCapturing failed");
-    return st != hipStreamCaptureStatusNone;
-}
-
-// Called on every eager call: creates the device's capture pool once, outside any capture.
-void ensure_capture_pool(const at::Tensor& like) {
-    const int dev = (int)like.device().index();
-    std::lock_guard<std::mutex> lk(g_mu);
-    if (!g_capture_pool.count(dev)) {
-        at::Tensor buf = torch::zeros({kCapturePoolSlots}, like.options().dtype(torch::kInt32));
-        // The zero fill runs on the current stream, and captured launches may later run on another
-        // one: wait for the fill alone, once per device, through an event (a stream or device
-        // synchronisation would invalidate a capture running on another stream in global mode).
-        hipEvent_t ev = nullptr;
-        TORCH_CHECK(hipEventCreateWithFlags(&ev, hipEventDisableTiming) == hipSuccess, "w4a16_gemm: hipEventCreate failed");
-        const bool ok = hipEventRecord(ev, c10::hip::getCurrentHIPStream(dev).stream()) == hipSuccess &&
-                        hipEventSynchronize(ev) == hipSuccess;
-        (void)hipEventDestroy(ev);
-        TORCH_CHECK(ok, "w4a16_gemm: waiting for the capture pool's zero fill failed");
-        g_capture_pool[dev].buf = buf;
-    }
-    if (dev >= 0 && dev < kMaxPoolDevices) g_pool_ready[dev].store(true, std::memory_order_release);
-}
-
-// Test hook: forget the capture pool of a device, so that the next call under capture takes the
-// no-pool path (counters zeroed by a fill kernel recorded in the graph).  The dropped buffer is
-// kept alive: graphs captured before the drop hold pointers into it and may still be replayed.
-std::vector<at::Tensor> g_dropped_pools;
-
-void drop_capture_pool(int64_t device) {
-    std::lock_guard<std::mutex> lk(g_mu);
-    auto it = g_capture_pool.find((int)device);
-    if (it == g_capture_pool.end()) return;
-    if (device >= 0 && device < kMaxPoolDevices) g_pool_ready[device].store(false, std::memory_order_release);
-    g_dropped_pools.push_back(it->second.buf);
-    g_capture_pool.erase(it);
-}
-
-at::Tensor split_counters(const at::Tensor& like, hipStream_t stream, int32_t slots) {
-    const auto opts = like.options().dtype(torch::kInt32);
-    const int dev = (int)like.device().index();
-    std::lock_guard<std::mutex> lk(g_mu);
-    if (capturing(stream)) {
-        auto pit = g_capture_pool.find(dev);
-        if (pit != g_capture_pool.end() && pit->second.next + slots <= kCapturePoolSlots) {
-            at::Tensor slice = pit->second.buf.narrow(0, pit->second.next, slots);
-            pit->second.next += (slots + 63) / 64 * 64;          // 256-byte aligned slices
-            return slice;
-        }
-        return torch::zeros({(int64_t)slots}, opts);
-    }
-    const std::pair<int, hipStream_t> key{dev, stream};
-    auto it = g_counters.find(key);
-    if (it == g_counters.end())
-        it = g_counters.emplace(key, torch::zeros({(int64_t)w4a16_max_counter_slots()}, opts)).first;
-    return it->second;
-}
 
 w4a16_device_limits limits_for(int dev) {
     w4a16_device_limits lim;
@@ -171,7 +76,7 @@ torch::Tensor w4a16_gemm(torch::Tensor Wp, torch::Tensor x, torch::Tensor scales
     torch::Tensor cnt_t;
     int32_t* cnt = nullptr;
     if (plan.counter_slots) {
-        cnt_t = split_counters(x, stream, plan.counter_slots);
+        cnt_t = split_counters(x, stream, plan.counter_slots, w4a16_max_counter_slots());
         cnt = cnt_t.data_ptr<int32_t>();
     }
 
