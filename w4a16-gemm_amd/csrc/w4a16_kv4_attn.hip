@@ -125,13 +125,15 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__
         bool there = false;                                  // the page is in the cache
         uint64_t kv = 0;
         int place = 0;
-        auto entry_at = [&](int tile) {
-            const int unit = ONE ? tile : tile * 4 + kb;
-            return units == 1 ? unit : (int)__umulhi((uint32_t)unit, page_magic);
-        };
-        auto entry = [&](int tile) { return tile * 64 + (ONE ? 0 : kb * 16) < kmax ? table[entry_at(tile)] : -1; };
-        auto aim = [&](int tile, int page) {
-            place = ONE ? (tile - entry_at(tile) * units) * 64 : (tile * 4 + kb - entry_at(tile) * units) * 16;
+        // Past the last key the last page's entry stands in: those tokens are masked.
+        auto unit_of = [&](int tile) { return ONE ? min(tile, (kmax - 1) >> 6) : min(tile * 4 + kb, (kmax - 1) >> 4); };
+        auto entry_at = [&](int unit) { return units == 1 ? unit : (int)__umulhi((uint32_t)unit, page_magic); };
+        // The table's entry stays in the lanes until a later turn uses it: made uniform at once, it would wait for every load.
+        const int nil = lane & 64;                           // 0, which the compiler does not know
+        auto entry = [&](int tile) { return table[entry_at(unit_of(tile)) + nil]; };
+        auto aim = [&](int tile, int entry) {
+            const int page = ONE ? __builtin_amdgcn_readfirstlane(entry) : entry, unit = unit_of(tile);
+            place = (unit - entry_at(unit) * units) * (ONE ? 64 : 16);
             there = (uint32_t)page < (uint32_t)a.c.pages;
             kv = (uint64_t)(uint32_t)(there ? page : 0) * a.c.page_bytes;
         };
@@ -167,9 +169,9 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__
         if (tile < stop) {
             aim(tile, entry(tile));
             load_sides();
+            page = entry(tile + WAVES);
             load_keys();
             load_values();
-            if (tile + WAVES < stop) page = entry(tile + WAVES);
         }
 
         // The rows' queries as digits, a wave to a row, while the first tile is on its way
@@ -251,7 +253,7 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__
             if (more) {
                 aim(tile + WAVES, page);
                 load_sides();
-                if (tile + 2 * WAVES < stop) page = entry(tile + 2 * WAVES);
+                page = entry(tile + 2 * WAVES);
             }
             {
                 int v = (int)big;
