@@ -81,7 +81,7 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
 // ONE: the page size is a multiple of 64, so a tile lies in one page and its addresses are the wave's.
 template <int D, int G, int NT, int WAVES, bool ONE>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 && D == G && WAVES == 4 ? 3 : NT <= 2 ? 2 : 1)))
-kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
+kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
     constexpr int NG = D / G, ROWS = 4 * NT, THREADS = 64 * WAVES;      // NG 2: groups of lower and of upper codes
     constexpr int NV = D / 32;                               // 16-byte pieces per lane of a value tile
     constexpr int kSide = NG * (64 * 8 + 128), kDigits = NT * NG * 1024;
@@ -94,11 +94,22 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__
     uint8_t* const side = lds + wave * (kSide + kDigits);
     uint8_t* const dig = side + kSide;
     const int units = ONE ? a.c.P >> 6 : a.c.P >> 4;         // tiles, or groups of 16 tokens, of a page
-    const int h = blockIdx.x % a.c.H, split = blockIdx.x / a.c.H, b = blockIdx.y;
+    const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;     // shares that only long sequences have come last
     const Kv4Seq s = kv4_seq(a, b);
     const int rows = s.count * a.rep, base = s.len - s.count;
     const int* const table = a.table + b * a.table_stride;
     const uint8_t* const mine = a.c.data + (uint64_t)(uint32_t)h * a.c.head_bytes;          // this head's bytes of page 0
+    // About how many tiles a workgroup takes if `groups` of them share all sequences' tiles: long ones are shared out, short
+    // ones not, whatever their lengths
+    int fair = 0;
+    if (splits > 1) {
+        for (int i = tid & 63; i < (int)gridDim.y; i += 64) {
+            const int n = max(a.lens[i], 0);
+            fair += ((a.window > 0 ? min(n, a.window + s.count) : n) + 63) >> 6;
+        }
+        fair = over_wave(fair, [](int p, int q) { return p + q; });
+        fair = (int)(((int64_t)fair * a.c.H + groups - 1) / groups);
+    }
 
     for (int row0 = 0; row0 < rows; row0 += ROWS) {
         const int first = row0 / a.rep, last = (min(row0 + ROWS, rows) - 1) / a.rep;
@@ -106,7 +117,12 @@ kv4_token_kernel(Kv4Attn a, int splits, uint32_t page_magic, float* __restrict__
         const int kmin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
         const int tile0 = kmin >> 6, tiles = a.c.pages > 0 ? max(0, ((kmax + 63) >> 6) - tile0) : 0;
         // more rows than one pass takes (max_q was too small for them) are not shared out
-        const int per = rows > ROWS ? max(tiles, 1) : max(WAVES, (tiles + splits - 1) / splits), parts = max(1, (tiles + per - 1) / per);
+        int per = max(tiles, 1), parts = 1;
+        if (rows <= ROWS) {
+            parts = min(splits, max(1, (tiles + max(WAVES, fair) - 1) / max(WAVES, fair)));
+            per = max(1, (tiles + parts - 1) / parts);
+            parts = max(1, (tiles + per - 1) / per);
+        }
         if (split >= parts) return;
         int lane = tid & 63;
         asm volatile("" : "+v"(lane));                       // what follows from it is not kept in registers across passes
@@ -941,7 +957,7 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
 // workgroups a sequence and head; both times `splits` shares of the keys, whose results the workspace holds.
 constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
 struct AttnPlan {
-    int nt, waves, row_tiles, splits;
+    int nt, waves, groups, row_tiles, splits;
     int64_t ml_at, o_at, bytes;
 };
 
@@ -954,8 +970,9 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
     if (rows <= 16) {
         p.nt = rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
         p.waves = p.nt <= 2 && items <= 64 && c.page_size % 64 == 0 ? 8 : 4;
-        const int64_t wanted = (p.waves == 8 ? 256 : 2048) / items;
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + p.waves - 1) / p.waves, W4A16_KV4_COUNTERS / items}));
+        p.groups = p.waves == 8 ? 256 : 768;
+        const int64_t most = (p.waves == 8 ? 256 : 2048) / items;
+        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (tiles + p.waves - 1) / p.waves, W4A16_KV4_COUNTERS / items}));
         if (p.splits > 1) {
             p.o_at = items * p.splits * 4 * p.nt * 8;
             p.bytes = p.o_at + items * p.splits * 4 * p.nt * c.head_dim * 4;
@@ -1024,10 +1041,10 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
         if (plan.nt) {
             const bool one = cache->page_size % 64 == 0;     // no tile of 64 tokens crosses a page
             const uint32_t magic = magic_of(cache->page_size / (one ? 64 : 16));
-            const dim3 grid((unsigned)(cache->kv_heads * plan.splits), (unsigned)args->batch);
+            const dim3 grid((unsigned)cache->kv_heads, (unsigned)args->batch, (unsigned)plan.splits);
             auto launch = [&](auto nt) {
                 auto on = [&](auto kernel, int waves) {
-                    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, plan.splits, magic, (float*)ws, po, counters);
+                    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, plan.splits, plan.groups, magic, (float*)ws, po, counters);
                 };
                 if constexpr (nt.value <= 2) {
                     if (plan.waves == 8) return on(kv4_token_kernel<d.value, g.value, nt.value, 8, true>, 8);
