@@ -420,6 +420,22 @@ def test_attention_of_sharp_and_flat_scores(q_len, dtype, size, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [3, 50])
+@pytest.mark.parametrize("D,G", SIZES)
+@pytest.mark.parametrize("least,most", [(-40, 0), (-9, 3), (-20, 100)])
+def test_attention_rows_of_very_different_sizes(q_len, D, G, least, most):
+    """One huge query costs the queries that share its workgroup nothing (bf16, whose range is beyond fp16's)."""
+    torch_cuda()
+    rng = np.random.default_rng(q_len + D + G + most)
+    cache, table = filled(rng, [200], 16, 2, D, G, torch.bfloat16)
+    size = 2.0 ** rng.integers(least, most + 1, (q_len, 4, 1))
+    size[0, 0], size[1, 0] = 2.0**most, 2.0**least
+    q = (values(rng, (q_len, 4, D), torch.float32) * torch.from_numpy(size).float()).to(torch.bfloat16)
+    out, lse, ref = attend(q, cache, table, [200], G, 16, [0, q_len], max_q=q_len)
+    check(out, lse, ref, torch.bfloat16)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["fused", "odd", "heads"])
 @pytest.mark.parametrize("q_len", [1, 50])
 def test_attention_takes_any_strides(layout, q_len):

@@ -41,6 +41,11 @@ __device__ __forceinline__ int over_wave(int v, F f) {
              f(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
+// A rounded product, which no later sum takes unrounded.
+__device__ __forceinline__ float times(float x, float y) {
+#pragma clang fp contract(off)
+    return x * y;
+}
 __device__ __forceinline__ void wave_lds_order() {           // a wave's own LDS operations stay in order
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -316,7 +321,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
                     float y = 0.f;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) y += fmaf(-zk[g], qsum[t][g], of_digits3(dot[g][0], dot[g][1], dot[g][2])) * sk[g];
-                    sc[t][r] = y;                            // times rs
+                    sc[t][r] = times(y, rs[t]);              // rounded before the largest is taken: p stays at most 1
                 }
             }
             __builtin_amdgcn_sched_barrier(0);               // not before this tile's are used: they take their registers
@@ -335,7 +340,6 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
                 }
                 float top = fmaxf(fmaxf(sc[t][0], sc[t][1]), fmaxf(sc[t][2], sc[t][3]));
                 W4A16_OVER_ROW(top, fmaxf);
-                top *= rs[t];
                 if (__any(top > m[t])) {
                     const float next = fmaxf(m[t], top);     // above -inf where m is
                     const float keep = next == m[t] ? 1.f : __builtin_amdgcn_exp2f(m[t] - next);
@@ -350,7 +354,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
                 const float safe = m[t] == -INFINITY ? 0.f : -m[t];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[t][r], rs[t], safe));
+                    const float p = __builtin_amdgcn_exp2f(sc[t][r] + safe);
                     l[t] += p;
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
