@@ -538,21 +538,35 @@ __device__ __forceinline__ uint32_t as_u32(h2 v) { return __builtin_bit_cast(uin
 
 // The eight codes of a dword less their zeros, in fp16: c | 0x6400 in bits 4..7 of a half is 1024 + 16 c, which one
 // FMA takes to c - z exactly (less = -64 - z).  lo0 and lo1 hold the lower codes of bytes 0, 2 and 1, 3, hi0 and hi1
-// the upper ones.
-__device__ __forceinline__ void expand(uint32_t w, h2 less_lo0, h2 less_lo1, h2 less_hi0, h2 less_hi1, uint32_t& lo0, uint32_t& lo1,
-                                       uint32_t& hi0, uint32_t& hi1) {
-    constexpr uint32_t mask = 0x00F000F0u, magic = 0x64006400u;
-    const h2 f = {(_Float16)0.0625f, (_Float16)0.0625f};
-    lo0 = as_u32(__builtin_elementwise_fma(as_h2(((w << 4) & mask) | magic), f, less_lo0));
-    hi0 = as_u32(__builtin_elementwise_fma(as_h2((w & mask) | magic), f, less_hi0));
-    lo1 = as_u32(__builtin_elementwise_fma(as_h2(((w >> 4) & mask) | magic), f, less_lo1));
-    hi1 = as_u32(__builtin_elementwise_fma(as_h2(((w >> 8) & mask) | magic), f, less_hi1));
-}
+// the upper ones.  The constants come in registers: mask and bits are one v_and_or_b32 only where at most one is a scalar.
+struct Expand {
+    uint32_t mask, magic;
+    h2 sixteenth;
+    __device__ __forceinline__ Expand() {
+        asm("s_mov_b32 %0, 0xf000f0" : "=s"(mask));
+        asm("v_mov_b32 %0, 0x64006400" : "=v"(magic));
+        uint32_t f;
+        asm("v_mov_b32 %0, 0x2c002c00" : "=v"(f));
+        sixteenth = as_h2(f);
+    }
+    __device__ __forceinline__ uint32_t two(uint32_t w, h2 less) const {
+        return as_u32(__builtin_elementwise_fma(as_h2((w & mask) | magic), sixteenth, less));
+    }
+    __device__ __forceinline__ void operator()(uint32_t w, h2 less_lo0, h2 less_lo1, h2 less_hi0, h2 less_hi1, uint32_t& lo0, uint32_t& lo1,
+                                               uint32_t& hi0, uint32_t& hi1) const {
+        lo0 = two(w << 4, less_lo0);
+        hi0 = two(w, less_hi0);
+        lo1 = two(w >> 4, less_lo1);
+        hi1 = two(w >> 8, less_hi1);
+    }
+};
 // -64 - z for two zeros; a NaN or anything past the format's range (which only unwritten places hold) becomes finite.
 __device__ __forceinline__ h2 less_of(uint32_t z) {
     const h2 most = {(_Float16)97.f, (_Float16)97.f}, base = {(_Float16)-64.f, (_Float16)-64.f};
     return base - __builtin_elementwise_min(__builtin_elementwise_max(as_h2(z), -most), most);
 }
+// x y, but 0 where either is 0, NaN times 0 too.
+__device__ float mul_zero(float x, float y) __asm("llvm.amdgcn.fmul.legacy");
 __device__ __forceinline__ float other_half(float v) {       // the value of lane ^ 32
     return __shfl_xor(v, 32, 64);
 }
@@ -562,8 +576,8 @@ __device__ __forceinline__ float other_half(float v) {       // the value of lan
 // scores (v_mfma_f32_32x32x16_f16: column lane % 32) and keeps that row's statistics to itself; its probabilities times
 // the values' scales are already where O^T = V^T P^T takes them from.  Scales are applied to the scores, so that only
 // the query (exact in fp16, a bf16 row times a power of two) and p s, rounded to fp16, are operands.
-// A row's reference `top` lies 2^7 under its largest score times the largest value scale seen: p s < 2^15 until that has
-// grown by 2^8, and only then are the sums scaled again.
+// Scores are kept less a row's reference `top`, so that one FMA makes them; p s < 2^15 holds until the largest has grown by
+// 2^8, and only then do the reference and the sums follow it.
 template <int D, int G, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
 kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
@@ -572,8 +586,9 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
     constexpr int kKeyRow = D * 2 + 16, kValRow = 144;       // LDS rows: a token's values; 64 tokens of one value
     constexpr int kVal = 64 * kKeyRow, kSk = kVal + D * kValRow, kSv = kSk + NG * 256, kEv = kSv + NG * 256, kBuf = kEv + 32;
     constexpr int kPieces = 64 * D / 32;                     // 16-byte pieces of a tile's keys, and of its values
-    static_assert(WAVES == 4, "a thread has one piece of keys and one of values, or waves 0 and 1 keys and 2 and 3 values");
-    constexpr int PER = D / 64;
+    static_assert(2 * kPieces == 256 * (D / 64) && (WAVES == 4 || (WAVES == 8 && D == 128)), "how pieces fall to threads");
+    constexpr int PER = 2 * kPieces / (64 * WAVES);          // 2: one of keys and one of values; 1: half the waves have keys
+    constexpr bool kGroups = D == 128;                       // a wave's pieces of values are of the same 16 tokens
     __shared__ __align__(16) uint8_t lds[2 * kBuf];
     const int tid = threadIdx.x, lane = tid & 63, half = lane >> 5, col = lane & 31;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -606,8 +621,10 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
         const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
 
         // The lane's query in fp16, values in the order of the keys' LDS rows: within four, 0 2 1 3
+        // (bf16: times a power of two that brings the workgroup's largest to 2^7 .. 2^8, which goes into the keys' scales; a row
+        // far from that has a power of its own, and its scores are taken times row_scale, so that no row costs another bits)
         h8 q[D / 16];
-        float rowf = 1.f;
+        float key_scale = a.scale2, row_scale = 1.f;
         {
             u4 w[D / 16];
             uint32_t big = 0;
@@ -631,23 +648,39 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 #pragma unroll
                 for (int j = 0; j < 8; ++j) big = max(big, __builtin_bit_cast(uint32_t, value(i, j)) & 0x7FFFFFFFu);
             big = max(big, (uint32_t)__shfl_xor((int)big, 32, 64));
+            const bool odd = big >= 0x7F800000u;
             int e = 0;
-            if (a.bf16) {                                    // the row's largest to 2^7 .. 2^8
-                e = big < 0x7F800000u ? min(max(__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, big)) - 8, -110), 110) : 0;
-                rowf = ldexpf(1.f, e);
+            if (a.bf16) {
+                const int most = over_wave(odd ? 0 : (int)big, [](int x, int y) { return max(x, y); });
+                int* const of_wave = reinterpret_cast<int*>(lds);
+                if (lane == 0) of_wave[wave] = most;
+                __syncthreads();
+                int all = of_wave[0];
+#pragma unroll
+                for (int i = 1; i < WAVES; ++i) all = max(all, of_wave[i]);
+                __syncthreads();
+                e = min(max(__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, all)) - 8, -110), 64);    // scores stay finite
+                key_scale = ldexpf(key_scale, e);
+                const int own = min(max(__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, big)) - 8, -110), 110);
+                if (!odd && big != 0 && (own < e - 10 || own > e)) {
+                    row_scale = ldexpf(1.f, own - e);
+                    e = own;
+                }
             }
-            if (big >= 0x7F800000u) rowf = NAN;
 #pragma unroll
             for (int i = 0; i < D / 16; ++i) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const int from = (j & 4) | ((j & 1) << 1) | ((j >> 1) & 1);
-                    q[i][j] = (_Float16)ldexpf(value(i, from), -e);
+                    q[i][j] = (_Float16)(a.bf16 ? ldexpf(value(i, from), -e) : value(i, from));
                 }
             }
+            if (odd) q[0][0] = (_Float16)NAN;                // whatever the infinities would make of it
         }
 
-        float top = -INFINITY, total = 0.f;
+        const bool uneven = __any(row_scale != 1.f);
+        float top = 0.f, total = 0.f;
+        bool fresh = true;                                   // the row has no scores yet
         f32x16 o[D / 32];
 #pragma unroll
         for (int i = 0; i < D / 32; ++i)
@@ -656,40 +689,47 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 
         // Each thread's pieces of a tile: 16 bytes of a token's keys, and of 16 tokens' values
         struct Piece {
-            u4 w, z[2][NG];
+            u4 w, z[kGroups ? 1 : 2][kGroups ? 1 : NG];
+            uint32_t zv[NG];
             uint16_t zk[NG], s[NG];
             bool there;
         };
-        auto keys = [&](int i) { return D == 128 ? i == 0 : wave < 2; };
-        const int p = D == 128 ? tid : tid & 127, mine = p / (kPieces / 4);
+        const Expand expand;
+        auto keys = [&](int i) { return PER == 2 ? i == 0 : wave < WAVES / 2; };
+        const int p = tid % kPieces, mine = kGroups ? wave & 3 : p / (kPieces / 4);
         auto entry = [&](int tile) {
             const int group = tile * 4 + mine;
             const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
             return group * 16 < kmax ? table[at] : -1;
         };
+        const uint32_t in = p % (D / 2);                     // which of the 16 tokens' pieces
         auto load = [&](int tile, int i, int page, Piece& x) {
+            if constexpr (kGroups) page = __builtin_amdgcn_readfirstlane(page);    // addresses: a scalar and a lane's part
             const int group = tile * 4 + mine;
             const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
             const int place = (group - at * groups) * 16;
             x.there = (uint32_t)page < (uint32_t)a.c.pages;
             const uint8_t* kv = a.c.head(x.there ? page : 0, h);
+            auto side = [&](int which, int g) { return kv + kv4_side<D, G>(a.c.P, which, g, place); };
             if (keys(i)) {
-                const int token = place + p / (D / 32) % 16;
-                x.w = *reinterpret_cast<const u4*>(kv + kv4_key_row<D>(token) + p % (D / 32) * 16);
+                x.w = *reinterpret_cast<const u4*>(kv + kv4_key_row<D>(place) + in * 16);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    x.zk[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, kKeyZero, g, token));
-                    x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, kKeyScale, g, token));
+                    x.zk[g] = *reinterpret_cast<const uint16_t*>(side(kKeyZero, g) + in / (D / 32) * 2);
+                    x.s[g] = *reinterpret_cast<const uint16_t*>(side(kKeyScale, g) + in / (D / 32) * 2);
                 }
             } else {
-                const int j = p % (D / 2);
-                x.w = *reinterpret_cast<const u4*>(kv + kv4_value_tile<D>(a.c.P, place) + j * 16);
+                x.w = *reinterpret_cast<const u4*>(kv + kv4_value_tile<D>(a.c.P, place) + in * 16);
 #pragma unroll
                 for (int g = 0; g < NG; ++g) {
-                    const u4* z = reinterpret_cast<const u4*>(kv + kv4_side<D, G>(a.c.P, kValueZero, g, place));
-                    x.z[0][g] = z[0];
-                    x.z[1][g] = z[1];
-                    x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, kValueScale, g, place + (j & 15)));
+                    const uint8_t* z = side(kValueZero, g);
+                    if constexpr (kGroups) {
+                        x.zv[g] = *reinterpret_cast<const uint32_t*>(z + in % 8 * 4);
+                    } else {
+                        x.z[0][g] = reinterpret_cast<const u4*>(z)[0];
+                        x.z[1][g] = reinterpret_cast<const u4*>(z)[1];
+                    }
+                    x.s[g] = *reinterpret_cast<const uint16_t*>(side(kValueScale, g) + in % 16 * 2);
                 }
             }
         };
@@ -719,17 +759,24 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
                     const bool live = x.there && tile * 64 + token < kmax;
 #pragma unroll
                     for (int g = 0; g < NG; ++g)
-                        *reinterpret_cast<float*>(buf + kSk + g * 256 + token * 4) = live ? half_bits(x.s[g]) * a.scale2 : 0.f;
+                        *reinterpret_cast<float*>(buf + kSk + g * 256 + token * 4) = live ? half_bits(x.s[g]) * key_scale : 0.f;
                 }
             } else {
                 const int j = p % (D / 2);
                 u4 l[2], u[2];                               // tokens 0-3 and 8-11, 4-7 and 12-15: a lane half's operand
+                uint32_t lz[NG];
+                if constexpr (kGroups) {
+#pragma unroll
+                    for (int g = 0; g < NG; ++g) lz[g] = as_u32(less_of(x.zv[g]));
+                }
+                auto less = [&](int g, int i) {              // of tokens 2 i and 2 i + 1
+                    if constexpr (kGroups) return as_h2(__builtin_amdgcn_readlane(lz[g], i));
+                    else return less_of(x.z[i >> 2][g][i & 3]);
+                };
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t z0 = x.z[i >> 1][0][2 * (i & 1)], z1 = x.z[i >> 1][0][2 * (i & 1) + 1];
-                    const uint32_t y0 = x.z[i >> 1][NG - 1][2 * (i & 1)], y1 = x.z[i >> 1][NG - 1][2 * (i & 1) + 1];
                     uint32_t a0, a1, b0, b1;
-                    expand(x.w[i], less_of(z0), less_of(z1), less_of(y0), less_of(y1), a0, a1, b0, b1);
+                    expand(x.w[i], less(0, 2 * i), less(0, 2 * i + 1), less(NG - 1, 2 * i), less(NG - 1, 2 * i + 1), a0, a1, b0, b1);
                     l[i & 1][i & 2] = a0;
                     l[i & 1][(i & 2) + 1] = a1;
                     u[i & 1][i & 2] = b0;
@@ -746,12 +793,12 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 #pragma unroll
                     for (int g = 0; g < NG; ++g) {
                         *reinterpret_cast<float*>(buf + kSv + g * 256 + (group * 16 + j) * 4) = live ? half_bits(x.s[g]) : 0.f;
-                        most = max(most, live ? min((int)x.s[g], 0x7BFF) : 0);
+                        most = max(most, live ? (int)x.s[g] : 0);
                     }
                     W4A16_OVER_ROW(most, max);
                     if (j == 0) {
-                        *reinterpret_cast<int*>(buf + kEv + group * 4) = (most >> 10) - 14;     // the scales are under 2^that
-                        *reinterpret_cast<int*>(buf + kEv + 16 + group * 4) = x.there;
+                        *reinterpret_cast<int*>(buf + kEv + group * 4) = (min(most, 0x7BFF) >> 10) - 14;   // the scales are under 2^that
+                        *reinterpret_cast<int*>(buf + kEv + 16 + group * 4) = (x.there ? 1 : 0) | (most > 0x7BFF ? 2 : 0);
                     }
                 }
             }
@@ -782,7 +829,8 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             other = now;
             if (tile < start || tile * 64 >= any_end || tile * 64 + 64 <= any_begin) continue;
 
-            f32x16 y[2];
+            f32x16 y[2];                                     // the scores less top
+            const float less_top = uneven ? 0.f : -top;
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
@@ -799,22 +847,29 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
                     for (int j = 0; j < 4; ++j) {
                         const f4 sk = *reinterpret_cast<const f4*>(now + kSk + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            y[tb][4 * j + i] = g == 0 ? acc[4 * j + i] * sk[i] : fmaf(acc[4 * j + i], sk[i], y[tb][4 * j + i]);
+                        for (int i = 0; i < 4; ++i) y[tb][4 * j + i] = fmaf(acc[4 * j + i], sk[i], g == 0 ? less_top : y[tb][4 * j + i]);
                     }
                     if constexpr (NG == 2) __builtin_amdgcn_sched_barrier(0);    // one set of sums at a time: registers
                 }
+            if (uneven) {
+#pragma unroll
+                for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y[tb][j] = fmaf(y[tb][j], row_scale, -top);
+            }
             const i4v evs = *reinterpret_cast<const i4v*>(now + kEv), flags = *reinterpret_cast<const i4v*>(now + kEv + 16);
             const int ev = max(max(evs[0], evs[1]), max(evs[2], evs[3]));
-            const bool there = __builtin_amdgcn_readfirstlane(flags[0] & flags[1] & flags[2] & flags[3]) != 0;
-            const bool whole = there && tile * 64 + 64 <= sure_end && tile * 64 >= sure_begin;
+            const int every = __builtin_amdgcn_readfirstlane(flags[0] & flags[1] & flags[2] & flags[3]);
+            const int any = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
+            const bool whole = (every & 1) && tile * 64 + 64 <= sure_end && tile * 64 >= sure_begin;
             if (!whole) {
+                const int here_end = end - tile * 64 - 4 * half, here_begin = begin - tile * 64 - 4 * half;
 #pragma unroll
                 for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) {
-                        const int at = tile * 64 + 4 * half + 32 * tb + 8 * (j >> 2) + (j & 3);
-                        const bool see = (int)(at < end) & (int)(at >= begin) & flags[2 * tb + (j >> 3)];
+                        const int at = 32 * tb + 8 * (j >> 2) + (j & 3);
+                        const bool see = (int)(at < here_end) & (int)(at >= here_begin) & flags[2 * tb + (j >> 3)];
                         y[tb][j] = see ? y[tb][j] : -INFINITY;
                     }
             }
@@ -823,46 +878,56 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) most = fmaxf(most, y[tb][j]);
-            most = fmaxf(most, other_half(most)) * rowf;
-            const float need = most + (float)(ev - 7);
-            if (__any(need > top + 8.f)) {                   // also where a row sees its first key: top is -inf
-                const float next = fmaxf(top, need);
-                const float keep = next == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - next);
-                top = next;
+            most = fmaxf(most, other_half(most));
+            // p s < 2^15; and a row's first scores, wherever they lie
+            const bool far = most > (float)(15 - ev) || (fresh && most > -INFINITY);
+            if (__any(far)) {
+                const float by = far ? most + (float)(ev - 7) : 0.f;
+                const float keep = fresh ? 1.f : __builtin_amdgcn_exp2f(-by);
+                fresh = fresh && !far;
+                top += by;
                 total *= keep;
 #pragma unroll
                 for (int i = 0; i < D / 32; ++i)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) o[i][j] *= keep;
+#pragma unroll
+                for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y[tb][j] -= by;
             }
-            const float safe = top == -INFINITY ? 0.f : -top;
+            // Products below take 0 times anything as 0, so a NaN scale of a token that a row does not see stays out of it.
+            // A token that it does see keeps a weight above 0 there.
+            if (any & 2) {
+#pragma unroll
+                for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) y[tb][j] = y[tb][j] < -120.f && y[tb][j] > -INFINITY ? -120.f : y[tb][j];
+            }
 #pragma unroll
             for (int tb = 0; tb < 2; ++tb) {
-                h8 ps[NG][2];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    f4 sv[NG];
-#pragma unroll
-                    for (int g = 0; g < NG; ++g) sv[g] = *reinterpret_cast<const f4*>(now + kSv + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e = __builtin_amdgcn_exp2f(fmaf(y[tb][4 * j + i], rowf, safe));
-                        total += e;
-#pragma unroll
-                        for (int g = 0; g < NG; ++g) {
-                            float v = e * sv[g][i];
-                            if (!whole && e == 0.f) v = 0.f;         // a token that another row sees may hold NaN
-                            ps[g][j >> 1][4 * (j & 1) + i] = (_Float16)v;
-                        }
-                    }
+                for (int j = 0; j < 16; ++j) {
+                    y[tb][j] = __builtin_amdgcn_exp2f(y[tb][j]);
+                    total += y[tb][j];
                 }
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i)
+                for (int g = 0; g < NG; ++g) {
+                    h8 ps[2];
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const h8 v = *reinterpret_cast<const h8*>(now + kVal + (32 * i + col) * kValRow + (2 * tb + k) * 32 + half * 16);
-                        o[i] = mfma32x32x16(v, ps[NG == 2 ? i / (D / 64) : 0][k], o[i]);
+                    for (int j = 0; j < 4; ++j) {
+                        const f4 sv = *reinterpret_cast<const f4*>(now + kSv + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) ps[j >> 1][4 * (j & 1) + i] = (_Float16)mul_zero(y[tb][4 * j + i], sv[i]);
                     }
+#pragma unroll
+                    for (int i = g * G / 32; i < (g + 1) * G / 32; ++i)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const h8 v = *reinterpret_cast<const h8*>(now + kVal + (32 * i + col) * kValRow + (2 * tb + k) * 32 + half * 16);
+                            o[i] = mfma32x32x16(v, ps[k], o[i]);
+                        }
+                }
             }
         }
 
@@ -892,7 +957,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
                         *reinterpret_cast<f4*>(part_o + share * D + 32 * i + 8 * j + 4 * half) =
                             f4{o[i][4 * j], o[i][4 * j + 1], o[i][4 * j + 2], o[i][4 * j + 3]};
                 if (half == 0) {
-                    part_ml[share] = float2{top, total};
+                    part_ml[share] = float2{total == 0.f ? -INFINITY : top, total};
                     if (split == 0) used[at] = parts;
                 }
             }
