@@ -1024,9 +1024,8 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
 
 // How a call runs.  The token kernel (nt: its rows are 4 nt, in workgroups of `waves`) or the prompt kernel on row_tiles
 // workgroups a sequence and head; both times `splits` shares of the keys, whose results the workspace holds.
-constexpr int kPromptWaves = 4, kPromptRows = 32 * kPromptWaves;
 struct AttnPlan {
-    int nt, waves, groups, row_tiles, splits;
+    int nt, waves, groups, row_tiles, splits;            // nt 0: the prompt kernel
     int64_t ml_at, o_at, bytes;
 };
 
@@ -1048,8 +1047,11 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
         }
         return p;
     }
-    p.row_tiles = (int)std::min<int64_t>((rows + kPromptRows - 1) / kPromptRows, 65535);
-    const int64_t wanted = 512 / (a.batch * c.kv_heads * p.row_tiles);
+    // 256 rows share a tile's staging where there are as many (128 values a head, 8192 tokens with themselves: 815 us with
+    // 128 rows, 742 with 256)
+    p.waves = c.head_dim == 128 && rows > 128 ? 8 : 4;
+    p.row_tiles = (int)std::min<int64_t>((rows + 32 * p.waves - 1) / (32 * p.waves), 65535);
+    const int64_t wanted = 2048 / p.waves / (a.batch * c.kv_heads * p.row_tiles);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + 3) / 4, 256}));
     if (p.splits > 1) {
         const int64_t all = a.tokens * a.heads;
@@ -1126,8 +1128,14 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
             else launch(std::integral_constant<int, 4>{});
         } else {
             const dim3 grid((unsigned)cache->kv_heads, (unsigned)(plan.row_tiles * plan.splits), (unsigned)args->batch);
-            hipLaunchKernelGGL((kv4_prompt_kernel<d.value, g.value, kPromptWaves>), grid, dim3(64 * kPromptWaves), 0, st, a, plan.row_tiles,
-                               plan.splits, magic_of(cache->page_size / 16), used, ml, po);
+            auto on = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, grid, dim3(64 * (unsigned)plan.waves), 0, st, a, plan.row_tiles, plan.splits,
+                                   magic_of(cache->page_size / 16), used, ml, po);
+            };
+            if constexpr (d.value == 128) {
+                if (plan.waves == 8) on(kv4_prompt_kernel<d.value, g.value, 8>);
+            }
+            if (plan.waves == 4) on(kv4_prompt_kernel<d.value, g.value, 4>);
             if (plan.splits > 1)
                 hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits,
                                    used, ml, po);
