@@ -567,8 +567,12 @@ __device__ __forceinline__ h2 less_of(uint32_t z) {
 }
 // x y, but 0 where either is 0, NaN times 0 too.
 __device__ float mul_zero(float x, float y) __asm("llvm.amdgcn.fmul.legacy");
-__device__ __forceinline__ float other_half(float v) {       // the value of lane ^ 32
-    return __shfl_xor(v, 32, 64);
+// Over lanes l and l ^ 32.
+template <class F>
+__device__ __forceinline__ float over_halves(float v, F f) {
+    const auto both = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v), false, false);
+    const uint32_t lower = both[0], upper = both[1];
+    return f(__builtin_bit_cast(float, lower), __builtin_bit_cast(float, upper));
 }
 
 // One workgroup takes 32 WAVES rows (query, query head) of one KV head and a share of their keys, in tiles of 64 that
@@ -829,28 +833,57 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             other = now;
             if (tile < start || tile * 64 >= any_end || tile * 64 + 64 <= any_begin) continue;
 
-            f32x16 y[2];                                     // the scores less top
+            // The order of products, LDS reads and vector instructions below is the one that they are issued in: an operand is
+            // read kAhead products before its own, and a block of scores is finished beside the next one's products.
+            constexpr int S = D / 16, GS = G / 16, F = 2 * S, kAhead = 4;
+            f32x16 y[2], acc[F / GS];                        // the scores less top; sums of a block of 32 tokens and a group
+            h8 k[F];
+            f4 sk[F / GS][4];
             const float less_top = uneven ? 0.f : -top;
+            auto key = [&](int f) { k[f] = *reinterpret_cast<const h8*>(now + (32 * (f / S) + col) * kKeyRow + f % S * 32 + half * 16); };
 #pragma unroll
-            for (int tb = 0; tb < 2; ++tb)
+            for (int f = 0; f < kAhead; ++f) key(f);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    f32x16 acc;
+            for (int f = 0; f <= F; ++f) {
+                const int block = f / GS, step = f % GS;
+                if (f < F) {
+                    if (step == 0) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) acc[j] = 0.f;
-#pragma unroll
-                    for (int i = g * G / 16; i < (g + 1) * G / 16; ++i) {
-                        const h8 k = *reinterpret_cast<const h8*>(now + (32 * tb + col) * kKeyRow + i * 32 + half * 16);
-                        acc = mfma32x32x16(k, q[i], acc);
+                        for (int j = 0; j < 16; ++j) acc[block][j] = 0.f;
                     }
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const f4 sk = *reinterpret_cast<const f4*>(now + kSk + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) y[tb][4 * j + i] = fmaf(acc[4 * j + i], sk[i], g == 0 ? less_top : y[tb][4 * j + i]);
+                    acc[block] = mfma32x32x16(k[f], q[f % S], acc[block]);
+                    if (f + kAhead < F) key(f + kAhead);
+                    if (step >= GS - 4) {
+                        const int j = step - (GS - 4);
+                        sk[block][j] = *reinterpret_cast<const f4*>(now + kSk + block % NG * 256 + (32 * (block / NG) + 8 * j + 4 * half) * 4);
                     }
-                    if constexpr (NG == 2) __builtin_amdgcn_sched_barrier(0);    // one set of sums at a time: registers
                 }
+                if (block > 0 && (f == F || step >= GS / 2)) {
+                    const int done = block - 1, tb = done / NG;
+#pragma unroll
+                    for (int j = f == F ? 0 : (step - GS / 2) * 32 / GS; j < (f == F ? 16 : (step - GS / 2 + 1) * 32 / GS); ++j)
+                        y[tb][j] = fmaf(acc[done][j], sk[done][j >> 2][j & 3], done % NG == 0 ? less_top : y[tb][j]);
+                }
+                if (f < F) __builtin_amdgcn_sched_barrier(0);
+            }
+            // and the first reads of the second product
+            h8 v[D / 8], ps[2][NG][2];
+            f4 sv[2][NG][4];
+            auto value_of = [&](int f) {
+                const int i = f % (D / 32), at = f / (D / 32);
+                v[f] = *reinterpret_cast<const h8*>(now + kVal + (32 * i + col) * kValRow + at * 32 + half * 16);
+            };
+            auto scales = [&](int tb, int j) {
+#pragma unroll
+                for (int g = 0; g < NG; ++g)
+                    sv[tb][g][j] = *reinterpret_cast<const f4*>(now + kSv + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
+            };
+#pragma unroll
+            for (int j = 0; j < 4; ++j) scales(0, j);
+#pragma unroll
+            for (int f = 0; f < kAhead; ++f) value_of(f);
+            scales(1, 0);
             if (uneven) {
 #pragma unroll
                 for (int tb = 0; tb < 2; ++tb)
@@ -878,7 +911,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
                 for (int j = 0; j < 16; ++j) most = fmaxf(most, y[tb][j]);
-            most = fmaxf(most, other_half(most));
+            most = over_halves(most, fmaxf);
             // p s < 2^15; and a row's first scores, wherever they lie
             const bool far = most > (float)(15 - ev) || (fresh && most > -INFINITY);
             if (__any(far)) {
@@ -904,34 +937,30 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 #pragma unroll
                     for (int j = 0; j < 16; ++j) y[tb][j] = y[tb][j] < -120.f && y[tb][j] > -INFINITY ? -120.f : y[tb][j];
             }
+            auto weigh = [&](int tb, int j) {
+                const float e = __builtin_amdgcn_exp2f(y[tb][j]);
+                total += e;
 #pragma unroll
-            for (int tb = 0; tb < 2; ++tb) {
+                for (int g = 0; g < NG; ++g) ps[tb][g][j >> 3][j & 7] = (_Float16)mul_zero(e, sv[tb][g][j >> 2][j & 3]);
+            };
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    y[tb][j] = __builtin_amdgcn_exp2f(y[tb][j]);
-                    total += y[tb][j];
+            for (int j = 0; j < 16; ++j) weigh(0, j);
+#pragma unroll
+            for (int f = 0; f < D / 8; ++f) {
+                const int i = f % (D / 32), at = f / (D / 32);
+                o[i] = mfma32x32x16(v[f], ps[at >> 1][NG == 2 ? i / (D / 64) : 0][at & 1], o[i]);
+                if (f + kAhead < D / 8) value_of(f + kAhead);
+                if (f < D / 16) {                            // the second 32 tokens' weights beside the first's products
+                    constexpr int E = 256 / D;
+                    if (f * E % 4 == 0 && f * E < 12) scales(1, f * E / 4 + 1);
+#pragma unroll
+                    for (int j = f * E; j < (f + 1) * E; ++j) weigh(1, j);
                 }
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    h8 ps[2];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const f4 sv = *reinterpret_cast<const f4*>(now + kSv + g * 256 + (32 * tb + 8 * j + 4 * half) * 4);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) ps[j >> 1][4 * (j & 1) + i] = (_Float16)mul_zero(y[tb][4 * j + i], sv[i]);
-                    }
-#pragma unroll
-                    for (int i = g * G / 32; i < (g + 1) * G / 32; ++i)
-#pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            const h8 v = *reinterpret_cast<const h8*>(now + kVal + (32 * i + col) * kValRow + (2 * tb + k) * 32 + half * 16);
-                            o[i] = mfma32x32x16(v, ps[k], o[i]);
-                        }
-                }
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
 
-        total += other_half(total);
+        total = over_halves(total, [](float a, float b) { return a + b; });
         if (row < rows) {
             const int64_t at = (int64_t)(s.first + query) * a.heads + head;
             if (parts == 1) {
