@@ -52,6 +52,7 @@ __device__ __forceinline__ float dpp(float v) {
 }
 constexpr int kXor1 = 0xB1, kXor2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;
 constexpr int kShiftDown = 0x100;            // + n: lane i gets lane i + n's, 0 past the row's end
+constexpr int kBroadcast = 0x150;            // + n: every lane of the row gets lane n's
 
 // 16-bit inputs and outputs, fp16 or bf16.
 __device__ __forceinline__ float load16(uint16_t b, bool bf16) {

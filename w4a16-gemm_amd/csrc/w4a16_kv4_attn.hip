@@ -692,56 +692,44 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             for (int j = 0; j < 16; ++j) o[i][j] = 0.f;
 
         // Each thread's pieces of a tile: 16 bytes of a token's keys, and of 16 tokens' values
+        // with the zeros of two tokens and one token's scales.  Keys and values come by the same instructions, none of them
+        // in a branch: what a branch leaves or takes is waited for where the branches meet, before it is needed.
         struct Piece {
-            u4 w, z[kGroups ? 1 : 2][kGroups ? 1 : NG];
-            uint32_t zv[NG];
-            uint16_t zk[NG], s[NG];
+            u4 w;
+            uint32_t zero[NG];
+            uint16_t s[NG];
             bool there;
         };
         const Expand expand;
         auto keys = [&](int i) { return PER == 2 ? i == 0 : wave < WAVES / 2; };
         const int p = tid % kPieces, mine = kGroups ? wave & 3 : p / (kPieces / 4);
-        auto entry = [&](int tile) {
-            const int group = tile * 4 + mine;
-            const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
-            return group * 16 < kmax ? table[at] : -1;
+        const uint32_t in = p % (D / 2), in_token = in / (D / 32);     // which of the 16 tokens' pieces, of keys their token
+        auto entry = [&](int tile) {                         // the last one for tiles past it
+            const int group = min(tile * 4 + mine, (kmax - 1) >> 4);
+            return table[groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic)];
         };
-        const uint32_t in = p % (D / 2);                     // which of the 16 tokens' pieces
         auto load = [&](int tile, int i, int page, Piece& x) {
             if constexpr (kGroups) page = __builtin_amdgcn_readfirstlane(page);    // addresses: a scalar and a lane's part
             const int group = tile * 4 + mine;
             const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
             const int place = (group - at * groups) * 16;
-            x.there = (uint32_t)page < (uint32_t)a.c.pages;
+            x.there = (uint32_t)page < (uint32_t)a.c.pages && group * 16 < kmax;
             const uint8_t* kv = a.c.head(x.there ? page : 0, h);
-            auto side = [&](int which, int g) { return kv + kv4_side<D, G>(a.c.P, which, g, place); };
-            if (keys(i)) {
-                x.w = *reinterpret_cast<const u4*>(kv + kv4_key_row<D>(place) + in * 16);
+            x.w = *reinterpret_cast<const u4*>(kv + (keys(i) ? kv4_key_row<D>(place) : kv4_value_tile<D>(a.c.P, place)) + in * 16);
 #pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    x.zk[g] = *reinterpret_cast<const uint16_t*>(side(kKeyZero, g) + in / (D / 32) * 2);
-                    x.s[g] = *reinterpret_cast<const uint16_t*>(side(kKeyScale, g) + in / (D / 32) * 2);
-                }
-            } else {
-                x.w = *reinterpret_cast<const u4*>(kv + kv4_value_tile<D>(a.c.P, place) + in * 16);
-#pragma unroll
-                for (int g = 0; g < NG; ++g) {
-                    const uint8_t* z = side(kValueZero, g);
-                    if constexpr (kGroups) {
-                        x.zv[g] = *reinterpret_cast<const uint32_t*>(z + in % 8 * 4);
-                    } else {
-                        x.z[0][g] = reinterpret_cast<const u4*>(z)[0];
-                        x.z[1][g] = reinterpret_cast<const u4*>(z)[1];
-                    }
-                    x.s[g] = *reinterpret_cast<const uint16_t*>(side(kValueScale, g) + in % 16 * 2);
-                }
+            for (int g = 0; g < NG; ++g) {
+                x.zero[g] = *reinterpret_cast<const uint32_t*>(kv + kv4_side<D, G>(a.c.P, keys(i) ? kKeyZero : kValueZero, g, place) +
+                                                               (keys(i) ? in_token / 2 : in % 8) * 4);
+                x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, keys(i) ? kKeyScale : kValueScale, g, place) +
+                                                            (keys(i) ? in_token : in % 16) * 2);
             }
         };
         auto put = [&](int tile, int i, const Piece& x, uint8_t* buf) {
             const int group = mine;
             if (keys(i)) {
                 const int token = p / (D / 32), c = p % (D / 32);
-                const h2 lo = less_of(x.zk[0] * 0x10001u), hi = less_of(x.zk[NG - 1] * 0x10001u);
+                auto less = [&](int g) { return less_of(__builtin_amdgcn_perm(0, x.zero[g], in_token & 1 ? 0x03020302u : 0x01000100u)); };
+                const h2 lo = less(0), hi = less(NG - 1);
                 u4 l0, l1, h0, h1;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -768,19 +756,19 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             } else {
                 const int j = p % (D / 2);
                 u4 l[2], u[2];                               // tokens 0-3 and 8-11, 4-7 and 12-15: a lane half's operand
-                uint32_t lz[NG];
-                if constexpr (kGroups) {
+                int mine_less[NG];                           // of tokens 2 (lane % 8) and the next
 #pragma unroll
-                    for (int g = 0; g < NG; ++g) lz[g] = as_u32(less_of(x.zv[g]));
-                }
-                auto less = [&](int g, int i) {              // of tokens 2 i and 2 i + 1
-                    if constexpr (kGroups) return as_h2(__builtin_amdgcn_readlane(lz[g], i));
-                    else return less_of(x.z[i >> 2][g][i & 3]);
-                };
+                for (int g = 0; g < NG; ++g) mine_less[g] = (int)as_u32(less_of(x.zero[g]));
+#define W4A16_LESS(g, i) as_h2((uint32_t)__builtin_amdgcn_update_dpp(0, mine_less[g], kBroadcast + (i), 0xF, 0xF, true))
+                const h2 l0[8] = {W4A16_LESS(0, 0), W4A16_LESS(0, 1), W4A16_LESS(0, 2), W4A16_LESS(0, 3),
+                                  W4A16_LESS(0, 4), W4A16_LESS(0, 5), W4A16_LESS(0, 6), W4A16_LESS(0, 7)};
+                const h2 l1[8] = {W4A16_LESS(NG - 1, 0), W4A16_LESS(NG - 1, 1), W4A16_LESS(NG - 1, 2), W4A16_LESS(NG - 1, 3),
+                                  W4A16_LESS(NG - 1, 4), W4A16_LESS(NG - 1, 5), W4A16_LESS(NG - 1, 6), W4A16_LESS(NG - 1, 7)};
+#undef W4A16_LESS
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t a0, a1, b0, b1;
-                    expand(x.w[i], less(0, 2 * i), less(0, 2 * i + 1), less(NG - 1, 2 * i), less(NG - 1, 2 * i + 1), a0, a1, b0, b1);
+                    expand(x.w[i], l0[2 * i], l0[2 * i + 1], l1[2 * i], l1[2 * i + 1], a0, a1, b0, b1);
                     l[i & 1][i & 2] = a0;
                     l[i & 1][(i & 2) + 1] = a1;
                     u[i & 1][i & 2] = b0;
@@ -816,7 +804,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 #pragma unroll
             for (int i = 0; i < PER; ++i) load(start, i, page, x[i]);
         }
-        if (start + 1 < stop) page = entry(start + 1);
+        if (start < stop) page = entry(start + 1);
         uint8_t *buf = lds, *other = lds + kBuf;
         for (int tile = start - 1; tile < stop; ++tile) {
             if (tile >= start) __syncthreads();              // this tile is in LDS, and nobody reads the other buffer
@@ -826,7 +814,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
                     put(tile + 1, i, x[i], other);
                     if (tile + 2 < stop) load(tile + 2, i, page, x[i]);
                 }
-                if (tile + 3 < stop) page = entry(tile + 3);
+                page = entry(tile + 3);
             }
             uint8_t* const now = buf;
             buf = other;
