@@ -983,38 +983,43 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
     }
 }
 
-// Joins the shares of one row (used[row] of them, each of its own part of the keys): one workgroup per row.
+// Joins the shares of one row (used[row] of them, each of its own part of the keys): a wave per row, whose lanes hold the
+// shares' statistics 64 at a time and two values of the result each.
 template <int D>
 __global__ void __launch_bounds__(256)
-kv4_join_kernel(Kv4Attn a, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml, const float* __restrict__ part_o) {
-    constexpr int Q = D / 4, R = 256 / Q;                    // threads of one share, shares at once
-    __shared__ float weight[256], sums[256];
-    __shared__ f4 acc[256];
-    const int64_t row = blockIdx.x;
-    const int parts = min(used[row], splits);
+kv4_join_kernel(Kv4Attn a, int64_t rows, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml,
+                const float* __restrict__ part_o) {
+    const int lane = threadIdx.x & 63;
+    const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row >= rows) return;
+    const int parts = __builtin_amdgcn_readfirstlane(min(used[row], splits));
     if (parts <= 1) return;
-    const int t = threadIdx.x;
-    const float2 ml = t < parts ? part_ml[row * splits + t] : float2{-INFINITY, 0.f};
-    weight[t] = ml.x;
-    __syncthreads();
+    const float2* const ml = part_ml + row * splits;
+    const float* const o = part_o + row * splits * D + 2 * lane % D;
     float top = -INFINITY;
-    for (int i = 0; i < parts; ++i) top = fmaxf(top, weight[i]);
-    const float f = __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
-    __syncthreads();
-    weight[t] = f;
-    sums[t] = f * ml.y;
-    __syncthreads();
-    float sum = 0.f;
-    for (int i = 0; i < parts; ++i) sum += sums[i];
-    f4 v = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-    for (int i = t / Q; i < parts; i += R) v += weight[i] * *reinterpret_cast<const f4*>(part_o + (row * splits + i) * D + t % Q * 4);
-    acc[t] = v;
-    __syncthreads();
-    if (t >= Q) return;
-    for (int i = 1; i < R; ++i) v += acc[i * Q + t];
-    kv4_finish<D>(a, row, 4 * t, top, sum, v[0], v[1]);
-    kv4_finish<D>(a, row, 4 * t + 2, top, sum, v[2], v[3]);
+    for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[i].x);
+    W4A16_OVER_ROW(top, fmaxf);
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = over_halves(top, fmaxf);
+    float sum = 0.f, v0 = 0.f, v1 = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        const float2 mine = i0 + lane < parts ? ml[i0 + lane] : float2{-INFINITY, 0.f};
+        const float f = __builtin_amdgcn_exp2f(mine.x - (top == -INFINITY ? 0.f : top)), l = f * mine.y;
+        const int n = min(64, parts - i0);
+        for (int i = 0; i < n; i += 8) {
+            float2 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const float2*>(o + (int64_t)(i0 + min(i + u, n - 1)) * D);
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), i + u));
+                sum += __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, l), i + u));
+                v0 = fmaf(w, i + u < n ? x[u].x : 0.f, v0);
+                v1 = fmaf(w, i + u < n ? x[u].y : 0.f, v1);
+            }
+        }
+    }
+    if (2 * lane < D) kv4_finish<D>(a, row, 2 * lane, top, sum, v0, v1);
 }
 
 static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_attention_args* a, const w4a16_device_limits* lim) {
@@ -1154,8 +1159,8 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
             }
             if (plan.waves == 4) on(kv4_prompt_kernel<d.value, g.value, 4>);
             if (plan.splits > 1)
-                hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)(args->tokens * args->heads)), dim3(256), 0, st, a, plan.splits,
-                                   used, ml, po);
+                hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)((args->tokens * args->heads + 3) / 4)), dim3(256), 0, st, a,
+                                   args->tokens * args->heads, plan.splits, used, ml, po);
         }
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_attention", hipGetErrorString(e));
