@@ -72,8 +72,8 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
     return float2{__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi)};
 }
 
-// A workgroup takes one KV head of one sequence and a share of its tiles of 64 keys, its waves a tile each in turn; 4 NT rows
-// (query, query head) at once.  The last of a head's workgroups to finish joins their results.
+// A workgroup takes 4 NT rows (query, query head) of one KV head of one sequence and a share of its tiles of 64 keys, its
+// waves a tile each in turn.  The last of a head's workgroups to finish joins their results.
 //
 // Both products run on v_mfma_i32_16x16x64_i8: the codes are its operand as they lie in the cache (a shift and a mask), the
 // other operand is a fixed-point number in digits, which fill the rows that four query heads leave of the 16: row 4 r + i
@@ -85,7 +85,7 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
 //
 // ONE: the page size is a multiple of 64, so a tile lies in one page and its addresses are the wave's.
 template <int D, int G, int NT, int WAVES, bool ONE>
-__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 && D == G && WAVES == 4 ? 3 : NT <= 2 ? 2 : 1)))
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 && D == G && WAVES == 4 ? 3 : 2)))
 kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
     constexpr int NG = D / G, ROWS = 4 * NT, THREADS = 64 * WAVES;      // NG 2: groups of lower and of upper codes
     constexpr int NV = D / 32;                               // 16-byte pieces per lane of a value tile
@@ -99,7 +99,8 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
     uint8_t* const side = lds + wave * (kSide + kDigits);
     uint8_t* const dig = side + kSide;
     const int units = ONE ? a.c.P >> 6 : a.c.P >> 4;         // tiles, or groups of 16 tokens, of a page
-    const int h = blockIdx.x, b = blockIdx.y, split = blockIdx.z;     // shares that only long sequences have come last
+    const int h = blockIdx.x % a.c.H, set = blockIdx.x / a.c.H, sets = gridDim.x / a.c.H;
+    const int b = blockIdx.y, split = blockIdx.z;            // shares that only long sequences have come last
     const Kv4Seq s = kv4_seq(a, b);
     const int rows = s.count * a.rep, base = s.len - s.count;
     const int* const table = a.table + b * a.table_stride;
@@ -113,17 +114,17 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
             fair += ((a.window > 0 ? min(n, a.window + s.count) : n) + 63) >> 6;
         }
         fair = over_wave(fair, [](int p, int q) { return p + q; });
-        fair = (int)(((int64_t)fair * a.c.H + groups - 1) / groups);
+        fair = (int)(((int64_t)fair * gridDim.x + groups - 1) / groups);
     }
 
-    for (int row0 = 0; row0 < rows; row0 += ROWS) {
+    for (int row0 = set * ROWS; row0 < rows; row0 += sets * ROWS) {
         const int first = row0 / a.rep, last = (min(row0 + ROWS, rows) - 1) / a.rep;
         const int kmax = a.causal ? max(0, min(base + last + 1, s.len)) : s.len;
         const int kmin = a.window > 0 ? max(0, base + first - a.window + 1) : 0;
         const int tile0 = kmin >> 6, tiles = a.c.pages > 0 ? max(0, ((kmax + 63) >> 6) - tile0) : 0;
-        // more rows than one pass takes (max_q was too small for them) are not shared out
+        // more rows than the sets of them take (max_q was too small for them) are not shared out
         int per = max(tiles, 1), parts = 1;
-        if (rows <= ROWS) {
+        if (rows <= sets * ROWS) {
             parts = min(splits, max(1, (tiles + max(WAVES, fair) - 1) / max(WAVES, fair)));
             per = max(1, (tiles + parts - 1) / parts);
             parts = max(1, (tiles + per - 1) / per);
@@ -428,7 +429,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
         }
         __syncthreads();
         auto row_at = [&](int r) { return (int64_t)(s.first + r / a.rep) * a.heads + h * a.rep + r % a.rep; };
-        const int64_t item = (int64_t)b * a.c.H + h, slot = item * splits + split;
+        const int64_t item = (int64_t)b * gridDim.x + blockIdx.x, slot = item * splits + split;
         for (int i = tid; i < ROWS * (D / 2); i += THREADS) {
             const int r = i / (D / 2), d = i % (D / 2) * 2;
             float top = jm[r];
@@ -451,7 +452,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
                 if (d == 0) put_shared(parts_ml + (slot * ROWS + r) * 2, top, sum);
             }
         }
-        if (parts > 1) {                                     // one pass only: rows <= ROWS
+        if (parts > 1) {                                     // one pass only
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (tid == 0) {
@@ -462,12 +463,12 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
             if (!last_one) return;
             // Four values a thread; sets of threads take the parts in turn and come together in LDS, always in one order.
             constexpr int Q = ROWS * D / 4, SETS = THREADS / Q > 1 ? THREADS / Q : 1, BATCH = 8;
-            const int set = SETS > 1 ? tid / Q : 0;
+            const int turn = SETS > 1 ? tid / Q : 0;
             float* const js = reinterpret_cast<float*>(lds);             // [SETS][Q][6]
             for (int i = SETS > 1 ? tid % Q : tid; i < Q; i += SETS > 1 ? Q : THREADS) {
                 const int r = i / (D / 4), d = i % (D / 4) * 4;
                 float top = -INFINITY, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int p0 = set; p0 < parts; p0 += SETS * BATCH) {
+                for (int p0 = turn; p0 < parts; p0 += SETS * BATCH) {
                     float2 ml[BATCH], x[BATCH], y[BATCH];
 #pragma unroll
                     for (int p = 0; p < BATCH; ++p) {
@@ -497,13 +498,13 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
                     }
                 }
                 if constexpr (SETS > 1) {
-                    float* const to = js + (set * Q + i) * 6;
+                    float* const to = js + (turn * Q + i) * 6;
                     to[0] = top;
                     to[1] = sum;
 #pragma unroll
                     for (int j = 0; j < 4; ++j) to[2 + j] = v[j];
                     __syncthreads();                         // one turn of the loop: every thread is here
-                    if (set > 0) return;
+                    if (turn > 0) return;
                     float next = -INFINITY;
 #pragma unroll
                     for (int w = 0; w < SETS; ++w) next = fmaxf(next, js[(w * Q + i) * 6]);
@@ -1053,13 +1054,17 @@ struct AttnPlan {
 
 static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attention_args& a, const w4a16_device_limits& lim) {
     AttnPlan p{};
-    const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep, items = a.batch * c.kv_heads;
+    const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep;
     int64_t tiles = (a.table_width * c.page_size + 63) / 64;
     if (a.window > 0) tiles = std::min(tiles, (a.window + a.max_q) / 64 + 2);
     p.splits = 1;
-    if (rows <= 16) {
-        p.nt = rows <= 4 ? 1 : rows <= 8 ? 2 : 4;
-        p.waves = p.nt <= 2 && items <= 64 && c.page_size % 64 == 0 ? 8 : 4;
+    // Up to 32 rows: the token kernel, 8 rows a workgroup (128 values in groups of 64, 8 KV heads, 64 sequences of 1000 to 4100
+    // keys: 16 rows 97 us, 24 130, 40 190; the prompt kernel 184, 184, 203.  4 sequences: 23, 28, 30; 25, 26, 29)
+    if (rows <= 32) {
+        p.nt = rows <= 4 ? 1 : 2;
+        p.row_tiles = (int)((rows + 4 * p.nt - 1) / (4 * p.nt));
+        const int64_t items = a.batch * c.kv_heads * p.row_tiles;
+        p.waves = items <= 64 && c.page_size % 64 == 0 ? 8 : 4;
         p.groups = p.waves == 8 ? 256 : 768;
         const int64_t most = (p.waves == 8 ? 256 : 2048) / items;
         p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (tiles + p.waves - 1) / p.waves, W4A16_KV4_COUNTERS / items}));
@@ -1134,20 +1139,17 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
         if (plan.nt) {
             const bool one = cache->page_size % 64 == 0;     // no tile of 64 tokens crosses a page
             const uint32_t magic = magic_of(cache->page_size / (one ? 64 : 16));
-            const dim3 grid((unsigned)cache->kv_heads, (unsigned)args->batch, (unsigned)plan.splits);
+            const dim3 grid((unsigned)(cache->kv_heads * plan.row_tiles), (unsigned)args->batch, (unsigned)plan.splits);
             auto launch = [&](auto nt) {
                 auto on = [&](auto kernel, int waves) {
                     hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, plan.splits, plan.groups, magic, (float*)ws, po, counters);
                 };
-                if constexpr (nt.value <= 2) {
-                    if (plan.waves == 8) return on(kv4_token_kernel<d.value, g.value, nt.value, 8, true>, 8);
-                }
-                if (one) on(kv4_token_kernel<d.value, g.value, nt.value, 4, true>, 4);
+                if (plan.waves == 8) on(kv4_token_kernel<d.value, g.value, nt.value, 8, true>, 8);
+                else if (one) on(kv4_token_kernel<d.value, g.value, nt.value, 4, true>, 4);
                 else on(kv4_token_kernel<d.value, g.value, nt.value, 4, false>, 4);
             };
             if (plan.nt == 1) launch(std::integral_constant<int, 1>{});
-            else if (plan.nt == 2) launch(std::integral_constant<int, 2>{});
-            else launch(std::integral_constant<int, 4>{});
+            else launch(std::integral_constant<int, 2>{});
         } else {
             const dim3 grid((unsigned)cache->kv_heads, (unsigned)(plan.row_tiles * plan.splits), (unsigned)args->batch);
             auto on = [&](auto kernel) {
