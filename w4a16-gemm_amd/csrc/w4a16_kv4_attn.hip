@@ -584,7 +584,7 @@ __device__ __forceinline__ float over_halves(float v, F f) {
 // Scores are kept less a row's reference `top`, so that one FMA makes them; p s < 2^15 holds until the largest has grown by
 // 2^8, and only then do the reference and the sums follow it.
 template <int D, int G, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(2, 2)))
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
                   float* __restrict__ part_o) {
     constexpr int NG = D / G, BM = 32 * WAVES;
@@ -621,8 +621,8 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
         const int any_begin = a.window > 0 ? max(0, base + wfirst - a.window + 1) : 0;
         const int sure_end = a.causal ? min(base + wfirst + 1, s.len) : s.len;
         const int sure_begin = a.window > 0 ? max(0, base + wlast - a.window + 1) : 0;
-        const int row = wr0 + col, query = row / a.rep, head = h * a.rep + row % a.rep, pos = base + query;
-        const int end = row < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
+        const int my_row = wr0 + col, pos = base + my_row / a.rep;
+        const int end = my_row < rows ? (a.causal ? min(pos + 1, s.len) : s.len) : 0;
         const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
 
         // The lane's query in fp16, values in the order of the keys' LDS rows: within four, 0 2 1 3
@@ -633,7 +633,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
         {
             u4 w[D / 16];
             uint32_t big = 0;
-            const int safe = min(row, rows - 1);             // rows past the last compute it again, unused
+            const int safe = min(my_row, rows - 1);             // rows past the last compute it again, unused
             const uint16_t* src = a.q + (int64_t)(s.first + safe / a.rep) * a.q_token + (int64_t)(h * a.rep + safe % a.rep) * a.q_head + 8 * half;
             if (a.q_wide) {
 #pragma unroll
@@ -665,7 +665,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
                 for (int i = 1; i < WAVES; ++i) all = max(all, of_wave[i]);
                 __syncthreads();
                 e = min(max(__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, all)) - 8, -110), 64);    // scores stay finite
-                key_scale = ldexpf(key_scale, e);
+                key_scale = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, ldexpf(key_scale, e))));
                 const int own = min(max(__builtin_amdgcn_frexp_expf(__builtin_bit_cast(float, big)) - 8, -110), 110);
                 if (!odd && big != 0 && (own < e - 10 || own > e)) {
                     row_scale = ldexpf(1.f, own - e);
@@ -704,7 +704,6 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
         const Expand expand;
         auto keys = [&](int i) { return PER == 2 ? i == 0 : wave < WAVES / 2; };
         const int p = tid % kPieces, mine = kGroups ? wave & 3 : p / (kPieces / 4);
-        const uint32_t in = p % (D / 2), in_token = in / (D / 32);     // which of the 16 tokens' pieces, of keys their token
         auto entry = [&](int tile) {                         // the last one for tiles past it
             const int group = min(tile * 4 + mine, (kmax - 1) >> 4);
             return table[groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic)];
@@ -715,13 +714,16 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             const int at = groups == 1 ? group : (int)__umulhi((uint32_t)group, page_magic);
             const int place = (group - at * groups) * 16;
             x.there = (uint32_t)page < (uint32_t)a.c.pages && group * 16 < kmax;
-            const uint8_t* kv = a.c.head(x.there ? page : 0, h);
-            x.w = *reinterpret_cast<const u4*>(kv + (keys(i) ? kv4_key_row<D>(place) : kv4_value_tile<D>(a.c.P, place)) + in * 16);
+            const uint8_t* kv = a.c.head(x.there ? page : 0, h) + place * 2;
+            uint32_t in = p % (D / 2);                       // which of the 16 tokens' pieces
+            asm volatile("" : "+v"(in));                     // its 64-bit offsets are not kept in registers
+            const uint32_t in_token = in / (D / 32);
+            x.w = *reinterpret_cast<const u4*>(kv + (keys(i) ? 0 : kv4_value_tile<D>(a.c.P, 0)) + place * (D / 2 - 2) + in * 16);
 #pragma unroll
             for (int g = 0; g < NG; ++g) {
-                x.zero[g] = *reinterpret_cast<const uint32_t*>(kv + kv4_side<D, G>(a.c.P, keys(i) ? kKeyZero : kValueZero, g, place) +
+                x.zero[g] = *reinterpret_cast<const uint32_t*>(kv + kv4_side<D, G>(a.c.P, keys(i) ? kKeyZero : kValueZero, g, 0) +
                                                                (keys(i) ? in_token / 2 : in % 8) * 4);
-                x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, keys(i) ? kKeyScale : kValueScale, g, place) +
+                x.s[g] = *reinterpret_cast<const uint16_t*>(kv + kv4_side<D, G>(a.c.P, keys(i) ? kKeyScale : kValueScale, g, 0) +
                                                             (keys(i) ? in_token : in % 16) * 2);
             }
         };
@@ -729,7 +731,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             const int group = mine;
             if (keys(i)) {
                 const int token = p / (D / 32), c = p % (D / 32);
-                auto less = [&](int g) { return less_of(__builtin_amdgcn_perm(0, x.zero[g], in_token & 1 ? 0x03020302u : 0x01000100u)); };
+                auto less = [&](int g) { return less_of(__builtin_amdgcn_perm(0, x.zero[g], token & 1 ? 0x03020302u : 0x01000100u)); };
                 const h2 lo = less(0), hi = less(NG - 1);
                 u4 l0, l1, h0, h1;
 #pragma unroll
@@ -824,7 +826,7 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 
             // The order of products, LDS reads and vector instructions below is the one that they are issued in: an operand is
             // read kAhead products before its own, and a block of scores is finished beside the next one's products.
-            constexpr int S = D / 16, GS = G / 16, F = 2 * S, kAhead = 4;
+            constexpr int S = D / 16, GS = G / 16, F = 2 * S, kAhead = D == 64 ? 2 : 4;
             f32x16 y[2], acc[F / GS];                        // the scores less top; sums of a block of 32 tokens and a group
             h8 k[F];
             f4 sk[F / GS][4];
@@ -949,6 +951,9 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             }
         }
 
+        int lane_end = tid & 63;
+        asm volatile("" : "+v"(lane_end));                   // the row is worked out again, not kept in registers
+        const int row = wr0 + lane_end % 32, query = row / a.rep, head = h * a.rep + row % a.rep, half = lane_end / 32;
         total = over_halves(total, [](float a, float b) { return a + b; });
         if (row < rows) {
             const int64_t at = (int64_t)(s.first + query) * a.heads + head;
@@ -1078,7 +1083,8 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
     // 128 rows, 742 with 256)
     p.waves = c.head_dim == 128 && rows > 128 ? 8 : 4;
     p.row_tiles = (int)std::min<int64_t>((rows + 32 * p.waves - 1) / (32 * p.waves), 65535);
-    const int64_t wanted = 2048 / p.waves / (a.batch * c.kv_heads * p.row_tiles);
+    // as many workgroups as run at once: three waves a SIMD with 64 values a head, two with 128
+    const int64_t wanted = (c.head_dim == 64 ? 3072 : 2048) / p.waves / (a.batch * c.kv_heads * p.row_tiles);
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({wanted, (tiles + 3) / 4, 256}));
     if (p.splits > 1) {
         const int64_t all = a.tokens * a.heads;
