@@ -42,6 +42,17 @@ __device__ __forceinline__ int kv4_run_start(uint64_t runs, int which) {
     return __ffsll((unsigned long long)runs) - 1;
 }
 
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+
+// x / N rounded once, for N whose reciprocal's rounding leaves a remainder that one FMA takes: over the reciprocal, and what is
+// left of x over it again (the correction step of a division by a correctly rounded reciprocal; 0 <= x < 2^17).
+template <int N>
+__device__ __forceinline__ float over_constant(float x) {
+    constexpr float r = 1.f / N;
+    const float q = x * r;
+    return fmaf(fmaf(-q, (float)N, x), r, q);
+}
+
 // Over the 8 or 16 lanes of a token's group of values.
 template <int LANES, typename T, class F>
 __device__ __forceinline__ T over_lanes(T v, F f) {
@@ -112,26 +123,40 @@ kv4_write_kernel(Kv4 c, const uint16_t* __restrict__ k, const uint16_t* __restri
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             float x[8];
-            int nan = 0;
-            float lo = INFINITY, hi = -INFINITY, before = 0.f;
+            u16x2 size = {0, 0};                             // the largest bits without their signs
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const uint32_t w = now[i][j >> 1];
-                const float y = load16((j & 1 ? w >> 16 : w) & 0xFFFF, BF16);
-                if (j & 1) nan |= __builtin_isunordered(y, before);
-                before = y;
-                x[j] = __builtin_amdgcn_fmed3f(y, -65504.f, 65504.f);
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = now[i][j];
+                x[2 * j] = load16(w & 0xFFFF, BF16);
+                x[2 * j + 1] = load16(w >> 16, BF16);
+                size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2, w & 0x7FFF7FFFu));
+            }
+            // past 65504, or no number: rarely in any of the wave's groups
+            int nan = 0;
+            if (__any(max(size.x, size.y) > (BF16 ? 0x477F : 0x7BFF))) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    nan |= x[j] != x[j];
+                    x[j] = __builtin_amdgcn_fmed3f(x[j], -65504.f, 65504.f);
+                }
+                nan = over_lanes<G / 8>(nan, [](int p, int q) { return p | q; });
+            }
+            float lo = x[0], hi = x[0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) {
                 lo = fminf(lo, x[j]);
                 hi = fmaxf(hi, x[j]);
             }
             lo = over_lanes<G / 8>(lo, [](float p, float q) { return fminf(p, q); });
             hi = over_lanes<G / 8>(hi, [](float p, float q) { return fmaxf(p, q); });
-            nan = over_lanes<G / 8>(nan, [](int p, int q) { return p | q; });
-            const float step = fmaxf(fmaxf((hi - lo) / 15.f, fmaxf(fabsf(lo), fabsf(hi)) / 96.f), 0x1p-14f);
+            const float step = fmaxf(fmaxf(over_constant<15>(hi - lo), over_constant<96>(fmaxf(fabsf(lo), fabsf(hi)))), 0x1p-14f);
             const float s = half_bits(to_half_bits(step));
-            const float z = rintf(-lo / s * 8.f) / 8.f;
-            constexpr float kMagic = 8388608.f;              // 2^23 + q has the code in its lowest byte
             const float rs = __builtin_amdgcn_rcpf(s);
+            // as for the codes below: |8 lo / s| <= 776, and 8 lo rs is within 2^-12 of it
+            float z = -lo * rs * 8.f;
+            if (fabsf(z - rintf(z)) > 0.5f - 0x1p-11f) z = -lo / s * 8.f;
+            z = rintf(z) / 8.f;
+            constexpr float kMagic = 8388608.f;              // 2^23 + q has the code in its lowest byte
             uint32_t q[8];
             float off = 0.f;                                 // how far the furthest value is from its code
 #pragma unroll
