@@ -436,6 +436,44 @@ def test_attention_rows_of_very_different_sizes(q_len, D, G, least, most):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("D,G", SIZES)
+@pytest.mark.parametrize("Hq,H,P,counts,window", [(8, 1, 16, [2, 2, 1, 2], 0), (8, 1, 64, [3, 1, 3, 0], 0), (16, 2, 64, [4, 4, 4, 4], 600),
+                                                  (8, 1, 32, [5, 2, 8, 1], 0), (4, 1, 16, [17, 3, 20, 1], 300)])
+def test_attention_shares_of_ragged_sequences(D, G, Hq, H, P, counts, window):
+    """8 to 80 rows, with and without sets of them, over contexts that workgroups share: every row once, from all its keys."""
+    torch_cuda()
+    rng = np.random.default_rng(D + G + sum(counts))
+    lens = [1300, 3, 740, 65]
+    cache, table = filled(rng, lens, P, H, D, G)
+    start = np.concatenate([[0], np.cumsum(counts)])
+    q = values(rng, (int(start[-1]), Hq, D), torch.float16)
+    out, lse, ref = attend(q, cache, table, lens, G, P, start, max_q=max(counts), window=window)
+    check(out, lse, ref, torch.float16)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [1, 6, 70])
+@pytest.mark.parametrize("D,G", SIZES)
+def test_attention_keeps_nan_of_no_weight(q_len, D, G):
+    """A value that is no number makes its group NaN for every row that sees it, however little its key weighs, and for no other."""
+    torch_cuda()
+    rng = np.random.default_rng(q_len + D)
+    P, n = 32, 150
+    k, v = (values(rng, (n, 1, D), torch.float16) for _ in range(2))
+    q = values(rng, (q_len, 2, D), torch.float16)
+    at = n - max(1, q_len // 2)                                  # seen by the later rows only
+    k[at] = -60 * q[-1, 0]                                       # at least for the last row its weight is 0 in fp32
+    v[at, 0, D - 1] = float("nan")
+    cache = np.zeros((5, 1, _kv4.page_bytes(P, D, G)), np.uint8)
+    _kv4.write(cache, k.float().numpy(), v.float().numpy(), np.arange(n), G, P)
+    table = np.arange(5, dtype=np.int32)[None]
+    out, _, _ = attend(q, cache, table, [n], G, P, [0, q_len], max_q=q_len)
+    sees = np.arange(n - q_len, n)[:, None, None] >= at
+    group = np.arange(D) // G == (D - 1) // G
+    assert np.array_equal(np.isnan(out.float().cpu().numpy()), np.broadcast_to(sees & group, out.shape))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["fused", "odd", "heads"])
 @pytest.mark.parametrize("q_len", [1, 50])
 def test_attention_takes_any_strides(layout, q_len):
