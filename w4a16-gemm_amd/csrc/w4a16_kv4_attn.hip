@@ -84,6 +84,15 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
 // off digit by digit: a value that is 0 weighs nothing however large p is.  The digits come together in fp32.
 //
 // ONE: the page size is a multiple of 64, so a tile lies in one page and its addresses are the wave's.
+//
+// Bound by memory where there is much of it: one token over 131072 keys of 8 heads of 128 values (142.6 MB) 32 us, 4.5 TB/s,
+// where reading these bytes in this order and nothing else takes 25; waves wait 66% of their cycles and the vector units are
+// busy for 36%.  64 sequences of 40 to 8192 keys in pages of 16 (108.6 MB) 39 us.  One token over 100 keys 5.1 us, two
+// launches' worth.  The digits cost matrix instructions, which are idle otherwise (6% here), and save widening 4-bit codes:
+// widened to fp16 they take about three vector instructions for two values, and their products' fp16 operands lose p's bits.
+// Waves of a workgroup do not share what they load, and 8 rows a workgroup are what registers hold at two waves a SIMD: with 16
+// there was one, and 64 sequences' 16 rows took 167 us instead of 97.  Eight waves where workgroups are few make one long
+// sequence's parts, and their join, half as many.
 template <int D, int G, int NT, int WAVES, bool ONE>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 && D == G && WAVES == 4 ? 3 : 2)))
 kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
@@ -583,6 +592,16 @@ __device__ __forceinline__ float over_halves(float v, F f) {
 // the query (exact in fp16, a bf16 row times a power of two) and p s, rounded to fp16, are operands.
 // Scores are kept less a row's reference `top`, so that one FMA makes them; p s < 2^15 holds until the largest has grown by
 // 2^8, and only then do the reference and the sums follow it.
+//
+// Bound by instruction issue: 8192 tokens with themselves (32 query heads on 8 KV heads of 128 values) 615 us, 895 TFLOP/s,
+// where an 8192^3 fp16 matrix product of a library reaches 1147.  Of a SIMD's cycles vector instructions take 56% and
+// matrix ones 41%; a wave and tile is 32 of these and about 280 of those, 32 exponentials among them.  512 queries over 16384
+// keys 159 us (849 TFLOP/s), of which the join is 10.  64 values a head have half the products for the same exponentials:
+// 8192 tokens of 16 heads 221 us, 620 TFLOP/s.
+// What made it: operands read ahead of their products in a written order (744 -> 673 us; the compiler's order waited for each),
+// staging loads that nothing waits for (645 -> 622), 256 rows to a tile's staging (815 -> 744).  Measured and not kept: staging
+// beside the products instead of before them, and the first weights taken before the largest score is known (both level or
+// slower: the waves of a SIMD fill each other's gaps already); the two halves of a tile to two waves where rows are few.
 template <int D, int G, int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2)))
 kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int* __restrict__ used, float2* __restrict__ part_ml,
@@ -990,7 +1009,8 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 }
 
 // Joins the shares of one row (used[row] of them, each of its own part of the keys): a wave per row, whose lanes hold the
-// shares' statistics 64 at a time and two values of the result each.
+// shares' statistics 64 at a time and two values of the result each.  512 queries of 32 heads, 4 shares: 9.6 us for 42 MB; a
+// workgroup per row with the shares' sums through LDS took 17.6.
 template <int D>
 __global__ void __launch_bounds__(256)
 kv4_join_kernel(Kv4Attn a, int64_t rows, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml,
