@@ -87,7 +87,7 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
 //
 // Bound by memory where there is much of it: one token over 131072 keys of 8 heads of 128 values (142.6 MB) 32 us, 4.5 TB/s,
 // where reading these bytes in this order and nothing else takes 25; waves wait 66% of their cycles and the vector units are
-// busy for 36%.  64 sequences of 40 to 8192 keys in pages of 16 (108.6 MB) 39 us.  One token over 100 keys 5.1 us, two
+// busy for 36%.  64 sequences of 40 to 8192 keys in pages of 16 (108.6 MB) 31 us.  One token over 100 keys 5.1 us, two
 // launches' worth.  The digits cost matrix instructions, which are idle otherwise (6% here), and save widening 4-bit codes:
 // widened to fp16 they take about three vector instructions for two values, and their products' fp16 operands lose p's bits.
 // Waves of a workgroup do not share what they load, and 8 rows a workgroup are what registers hold at two waves a SIMD: with 16
@@ -95,7 +95,7 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
 // sequence's parts, and their join, half as many.
 template <int D, int G, int NT, int WAVES, bool ONE>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(NT == 1 && D == G && WAVES == 4 ? 3 : 2)))
-kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
+kv4_token_kernel(Kv4Attn a, int batch, int groups, uint32_t page_magic, float* __restrict__ parts_ml, float* __restrict__ parts_o, int* __restrict__ counters) {
     constexpr int NG = D / G, ROWS = 4 * NT, THREADS = 64 * WAVES;      // NG 2: groups of lower and of upper codes
     constexpr int NV = D / 32;                               // 16-byte pieces per lane of a value tile
     constexpr int kSide = NG * (64 * 8 + 128), kDigits = NT * NG * 1024;
@@ -109,22 +109,56 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
     uint8_t* const dig = side + kSide;
     const int units = ONE ? a.c.P >> 6 : a.c.P >> 4;         // tiles, or groups of 16 tokens, of a page
     const int h = blockIdx.x % a.c.H, set = blockIdx.x / a.c.H, sets = gridDim.x / a.c.H;
-    const int b = blockIdx.y, split = blockIdx.z;            // shares that only long sequences have come last
+    // blockIdx.y: the sequences' shares one after another, as many of each as its length has of `fair` tiles, the share of a
+    // workgroup if `groups` of them had all tiles alike, in whole turns of its waves.  Every workgroup finds its own by a sum
+    // over the lengths.  (64 sequences of 40 to 8192 keys: 31 us; at most four shares a sequence, which left 32 tiles to those
+    // of the longest, 39.)
+    int b = blockIdx.y, split = 0, shares = 1;
+    if ((int)gridDim.y > batch) {
+        const int lane = tid & 63;
+        auto tiles_of = [&](int i) {
+            int n = i < batch ? (int)min((int64_t)max(a.lens[i], 0), (int64_t)a.width * a.c.P) : 0;
+            if (a.window > 0 && n - a.window > 64) n = a.window + 64;
+            return (n + 63) >> 6;
+        };
+        int total = 0;
+        if (batch == 1) {
+            total = tiles_of(0);
+        } else {
+            for (int i = lane; i < batch; i += 64) total += tiles_of(i);
+            total = over_wave(total, [](int p, int q) { return p + q; });
+        }
+        const int fair = max(WAVES, ((int)(((int64_t)total * gridDim.x + groups - 1) / groups) + WAVES - 1) / WAVES * WAVES);
+        int before = 0;
+        b = batch;
+        if (batch == 1) {                                    // no sum to take
+            split = (int)blockIdx.y;
+            shares = max(1, (total + fair - 1) / fair);
+            b = split < shares ? 0 : 1;
+        }
+        for (int i0 = 0; batch > 1 && i0 < batch && b == batch; i0 += 64) {
+            const int own = i0 + lane < batch ? max(1, (tiles_of(i0 + lane) + fair - 1) / fair) : 0;
+            int upto = own;                                  // with the lanes below
+#pragma unroll
+            for (int d = 1; d < 64; d *= 2) {
+                const int below = __shfl_up(upto, d, 64);
+                upto += lane >= d ? below : 0;
+            }
+            const uint64_t past = __ballot(before + upto > (int)blockIdx.y);
+            if (past) {
+                const int at = __ffsll((unsigned long long)past) - 1;
+                b = i0 + at;
+                shares = __builtin_amdgcn_readlane(own, at);
+                split = (int)blockIdx.y - (before + __builtin_amdgcn_readlane(upto, at) - shares);
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
+        }
+        if (b == batch) return;                              // there are fewer shares than workgroups
+    }
     const Kv4Seq s = kv4_seq(a, b);
     const int rows = s.count * a.rep, base = s.len - s.count;
     const int* const table = a.table + b * a.table_stride;
     const uint8_t* const mine = a.c.data + (uint64_t)(uint32_t)h * a.c.head_bytes;          // this head's bytes of page 0
-    // About how many tiles a workgroup takes if `groups` of them share all sequences' tiles: long ones are shared out, short
-    // ones not, whatever their lengths
-    int fair = 0;
-    if (splits > 1) {
-        for (int i = tid & 63; i < (int)gridDim.y; i += 64) {
-            const int n = max(a.lens[i], 0);
-            fair += ((a.window > 0 ? min(n, a.window + s.count) : n) + 63) >> 6;
-        }
-        fair = over_wave(fair, [](int p, int q) { return p + q; });
-        fair = (int)(((int64_t)fair * gridDim.x + groups - 1) / groups);
-    }
 
     for (int row0 = set * ROWS; row0 < rows; row0 += sets * ROWS) {
         const int first = row0 / a.rep, last = (min(row0 + ROWS, rows) - 1) / a.rep;
@@ -134,8 +168,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
         // more rows than the sets of them take (max_q was too small for them) are not shared out
         int per = max(tiles, 1), parts = 1;
         if (rows <= sets * ROWS) {
-            parts = min(splits, max(1, (tiles + max(WAVES, fair) - 1) / max(WAVES, fair)));
-            per = max(1, (tiles + parts - 1) / parts);
+            per = max(1, (tiles + shares - 1) / shares);
             parts = max(1, (tiles + per - 1) / per);
         }
         if (split >= parts) return;
@@ -438,7 +471,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
         }
         __syncthreads();
         auto row_at = [&](int r) { return (int64_t)(s.first + r / a.rep) * a.heads + h * a.rep + r % a.rep; };
-        const int64_t item = (int64_t)b * gridDim.x + blockIdx.x, slot = item * splits + split;
+        const int64_t slot = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;    // a sequence's shares are gridDim.x apart
         for (int i = tid; i < ROWS * (D / 2); i += THREADS) {
             const int r = i / (D / 2), d = i % (D / 2) * 2;
             float top = jm[r];
@@ -465,8 +498,9 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             if (tid == 0) {
-                last_one = __hip_atomic_fetch_add(counters + item, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
-                if (last_one) __hip_atomic_store(counters + item, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                int* const counter = counters + (int64_t)b * gridDim.x + blockIdx.x;
+                last_one = __hip_atomic_fetch_add(counter, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+                if (last_one) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
             __syncthreads();
             if (!last_one) return;
@@ -481,7 +515,7 @@ kv4_token_kernel(Kv4Attn a, int splits, int groups, uint32_t page_magic, float* 
                     float2 ml[BATCH], x[BATCH], y[BATCH];
 #pragma unroll
                     for (int p = 0; p < BATCH; ++p) {
-                        const int64_t from = (item * splits + min(p0 + p * SETS, parts - 1)) * ROWS + r;
+                        const int64_t from = (slot + (int64_t)(min(p0 + p * SETS, parts - 1) - split) * gridDim.x) * ROWS + r;
                         ml[p] = get_shared(parts_ml + from * 2);
                         x[p] = get_shared(parts_o + from * D + d);
                         y[p] = get_shared(parts_o + from * D + d + 2);
@@ -1084,18 +1118,21 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
     if (a.window > 0) tiles = std::min(tiles, (a.window + a.max_q) / 64 + 2);
     p.splits = 1;
     // Up to 32 rows: the token kernel, 8 rows a workgroup (128 values in groups of 64, 8 KV heads, 64 sequences of 1000 to 4100
-    // keys: 16 rows 97 us, 24 130, 40 190; the prompt kernel 184, 184, 203.  4 sequences: 23, 28, 30; 25, 26, 29)
+    // keys: 16 rows 105 us, 24 132, 32 162, 40 195; the prompt kernel 184, 184, 201, 201.  4 sequences: 17, 18, 20, 29; 25, 26,
+    // 28, 29.  One of 50000: 40 rows 82; 58)
     if (rows <= 32) {
         p.nt = rows <= 4 ? 1 : 2;
         p.row_tiles = (int)((rows + 4 * p.nt - 1) / (4 * p.nt));
         const int64_t items = a.batch * c.kv_heads * p.row_tiles;
         p.waves = items <= 64 && c.page_size % 64 == 0 ? 8 : 4;
-        p.groups = p.waves == 8 ? 256 : 768;
-        const int64_t most = (p.waves == 8 ? 256 : 2048) / items;
-        p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({most, (tiles + p.waves - 1) / p.waves, W4A16_KV4_COUNTERS / items}));
-        if (p.splits > 1) {
-            p.o_at = items * p.splits * 4 * p.nt * 8;
-            p.bytes = p.o_at + items * p.splits * 4 * p.nt * c.head_dim * 4;
+        p.groups = p.waves == 8 ? 256 : 512;
+        const int64_t across = c.kv_heads * p.row_tiles;
+        p.splits = (int)a.batch;                             // workgroups down the grid: a share of a sequence each
+        if (items <= W4A16_KV4_COUNTERS)
+            p.splits = (int)std::min<int64_t>(a.batch + (p.groups + across - 1) / across, a.batch * std::max<int64_t>(1, (tiles + p.waves - 1) / p.waves));
+        if (p.splits > a.batch) {
+            p.o_at = across * p.splits * 4 * p.nt * 8;
+            p.bytes = p.o_at + across * p.splits * 4 * p.nt * c.head_dim * 4;
         }
         return p;
     }
@@ -1165,10 +1202,10 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
         if (plan.nt) {
             const bool one = cache->page_size % 64 == 0;     // no tile of 64 tokens crosses a page
             const uint32_t magic = magic_of(cache->page_size / (one ? 64 : 16));
-            const dim3 grid((unsigned)(cache->kv_heads * plan.row_tiles), (unsigned)args->batch, (unsigned)plan.splits);
+            const dim3 grid((unsigned)(cache->kv_heads * plan.row_tiles), (unsigned)plan.splits);
             auto launch = [&](auto nt) {
                 auto on = [&](auto kernel, int waves) {
-                    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, plan.splits, plan.groups, magic, (float*)ws, po, counters);
+                    hipLaunchKernelGGL(kernel, grid, dim3(64 * waves), 0, st, a, (int)args->batch, plan.groups, magic, (float*)ws, po, counters);
                 };
                 if (plan.waves == 8) on(kv4_token_kernel<d.value, g.value, nt.value, 8, true>, 8);
                 else if (one) on(kv4_token_kernel<d.value, g.value, nt.value, 4, true>, 4);
