@@ -940,15 +940,17 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
             const int any = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
             const bool whole = (every & 1) && tile * 64 + 64 <= sure_end && tile * 64 >= sure_begin;
             if (!whole) {
+                // one comparison a score for each of the edges that cross the tile
                 const int here_end = end - tile * 64 - 4 * half, here_begin = begin - tile * 64 - 4 * half;
+                auto keep = [&](auto see) {
 #pragma unroll
-                for (int tb = 0; tb < 2; ++tb)
+                    for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const int at = 32 * tb + 8 * (j >> 2) + (j & 3);
-                        const bool see = (int)(at < here_end) & (int)(at >= here_begin) & flags[2 * tb + (j >> 3)];
-                        y[tb][j] = see ? y[tb][j] : -INFINITY;
-                    }
+                        for (int j = 0; j < 16; ++j) y[tb][j] = see(tb, j) ? y[tb][j] : -INFINITY;
+                };
+                if (tile * 64 + 64 > sure_end) keep([&](int tb, int j) { return 32 * tb + 8 * (j >> 2) + (j & 3) < here_end; });
+                if (tile * 64 < sure_begin) keep([&](int tb, int j) { return 32 * tb + 8 * (j >> 2) + (j & 3) >= here_begin; });
+                if (!(every & 1)) keep([&](int tb, int j) { return (flags[2 * tb + (j >> 3)] & 1) != 0; });
             }
             float most = y[0][0];
 #pragma unroll
