@@ -1106,8 +1106,9 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
     return nullptr;
 }
 
-// How a call runs.  The token kernel (nt: its rows are 4 nt, in workgroups of `waves`) or the prompt kernel on row_tiles
-// workgroups a sequence and head; both times `splits` shares of the keys, whose results the workspace holds.
+// How a call runs.  The token kernel: workgroups of `waves` for 4 nt rows, row_tiles sets of them, `splits` down the grid for
+// all sequences' shares of about `groups` workgroups in all.  Or the prompt kernel: row_tiles workgroups a sequence and head,
+// for each `splits` shares of the keys.  The workspace holds the shares' results.
 struct AttnPlan {
     int nt, waves, groups, row_tiles, splits;            // nt 0: the prompt kernel
     int64_t ml_at, o_at, bytes;
@@ -1118,7 +1119,6 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
     const int64_t rep = a.heads / c.kv_heads, rows = a.max_q * rep;
     int64_t tiles = (a.table_width * c.page_size + 63) / 64;
     if (a.window > 0) tiles = std::min(tiles, (a.window + a.max_q) / 64 + 2);
-    p.splits = 1;
     // Up to 32 rows: the token kernel, 8 rows a workgroup (128 values in groups of 64, 8 KV heads, 64 sequences of 1000 to 4100
     // keys: 16 rows 105 us, 24 132, 32 162, 40 195; the prompt kernel 184, 184, 201, 201.  4 sequences: 17, 18, 20, 29; 25, 26,
     // 28, 29.  One of 50000: 40 rows 82; 58)
@@ -1126,6 +1126,7 @@ static AttnPlan plan_attention(const w4a16_kv4_cache& c, const w4a16_kv4_attenti
         p.nt = rows <= 4 ? 1 : 2;
         p.row_tiles = (int)((rows + 4 * p.nt - 1) / (4 * p.nt));
         const int64_t items = a.batch * c.kv_heads * p.row_tiles;
+        // as many workgroups as run at once; eight waves where heads are few, so that the shares to join are half as many
         p.waves = items <= 64 && c.page_size % 64 == 0 ? 8 : 4;
         p.groups = p.waves == 8 ? 256 : 512;
         const int64_t across = c.kv_heads * p.row_tiles;
