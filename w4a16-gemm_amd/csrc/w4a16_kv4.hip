@@ -207,7 +207,8 @@ kv4_write_kernel(Kv4 c, const uint16_t* __restrict__ k, const uint16_t* __restri
 // Lane l of a token gives values 8 l .. 8 l + 7: the lower codes of eight bytes, or (from D/2 on) the upper ones of the same.
 // q - z is exact in fp16 (1024 + 16 q times 1/16 less 64 + z), and so its product with s needs one rounding.
 // Bound by its writes: 32768 tokens of 8 heads of 128 values (35.7 MB read, 134 written) 37 to 41 us, 4.1 to 4.6 TB/s, where a copy
-// reaches 5.1; 8192 tokens 13.6 us, 2.8 TB/s, two rounds of workgroups of which the first waits for its slots.
+// reaches 5.1; 8192 tokens 13.2 us, 2.8 TB/s, two rounds of workgroups of which the first waits for its slots.  Nontemporal
+// stores end the large call after 27 us, but an addition that then takes both outputs needs 17 more: 68 us for both, not 61.
 template <int D, int G, int W, bool BF16>
 __global__ void __launch_bounds__(W * D / 8)
 kv4_read_kernel(Kv4 c, const int64_t* __restrict__ slots, int tokens, uint16_t* __restrict__ k, uint16_t* __restrict__ v) {
@@ -275,7 +276,10 @@ kv4_read_kernel(Kv4 c, const int64_t* __restrict__ slots, int tokens, uint16_t* 
                 if constexpr (!BF16) {
                     out[j] = __builtin_bit_cast(uint32_t, code * scale);
                 } else {
-                    out[j] = (uint32_t)store16((float)code[0] * (float)scale[0], 1) | ((uint32_t)store16((float)code[1] * (float)scale[1], 1) << 16);
+                    typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+                    typedef float fl2 __attribute__((ext_vector_type(2)));
+                    const fl2 y = {(float)code[0] * (float)scale[0], (float)code[1] * (float)scale[1]};
+                    out[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector(y, bf2));
                 }
             }
             if (t < here) *reinterpret_cast<u4*>((i ? v : k) + ((first + t) * c.H + h) * D + 8 * l) = live ? out : u4{0, 0, 0, 0};

@@ -85,10 +85,10 @@ __device__ __forceinline__ float2 get_shared(const float* p) {
 //
 // ONE: the page size is a multiple of 64, so a tile lies in one page and its addresses are the wave's.
 //
-// Bound by memory where there is much of it: one token over 131072 keys of 8 heads of 128 values (142.6 MB) 32 us, 4.5 TB/s,
+// Bound by memory where there is much of it: one token over 131072 keys of 8 heads of 128 values (142.6 MB) 29 us, 4.9 TB/s,
 // where reading these bytes in this order and nothing else takes 25; waves wait 66% of their cycles and the vector units are
-// busy for 36%.  64 sequences of 40 to 8192 keys in pages of 16 (108.6 MB) 31 us.  One token over 100 keys 5.1 us, two
-// launches' worth.  The digits cost matrix instructions, which are idle otherwise (6% here), and save widening 4-bit codes:
+// busy for 36%.  64 sequences of 40 to 8192 keys in pages of 16 (108.6 MB) 30 us.  One token over 100 keys 5.1 us, a
+// launch and four dependent loads.  The digits cost matrix instructions, which are idle otherwise (6% here), and save widening 4-bit codes:
 // widened to fp16 they take about three vector instructions for two values, and their products' fp16 operands lose p's bits.
 // Waves of a workgroup do not share what they load, and 8 rows a workgroup are what registers hold at two waves a SIMD: with 16
 // there was one, and 64 sequences' 16 rows took 167 us instead of 97.  Eight waves where workgroups are few make one long
@@ -209,6 +209,8 @@ kv4_token_kernel(Kv4Attn a, int batch, int groups, uint32_t page_magic, float* _
                 for (int g = 0; g < NG; ++g)
                     sides[w][g] = *reinterpret_cast<const uint16_t*>(at + kv4_side<D, G>(a.c.P, w, g, 0) + (uint32_t)((ONE ? lane : n) * 2));
         };
+        // Codes are used once a call: nontemporal loads (131072 keys 31.9 -> 29.1 us, 64 sequences of 2048 29.6 -> 26.8; level
+        // where sets of rows read them again; 4096 keys that the last call left in L2 9.4 -> 9.9)
         auto load_keys = [&] {
             const uint64_t at = kv + kv4_key_row<D>(place);
 #pragma unroll
@@ -218,14 +220,14 @@ kv4_token_kernel(Kv4Attn a, int batch, int groups, uint32_t page_magic, float* _
                 if constexpr (!ONE)
                     row = ((uint64_t)__builtin_amdgcn_readlane((uint32_t)(at >> 32), 16 * r) << 32) |
                           __builtin_amdgcn_readlane((uint32_t)at, 16 * r);
-                k[r] = *reinterpret_cast<const u4*>(mine + row + off);
+                k[r] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(mine + row + off));
             }
         };
         auto load_values = [&] {
             const uint8_t* vals = mine + kv + kv4_value_tile<D>(a.c.P, place);
             const uint32_t off = n * 16 + (ONE ? kb * (D / 2 * 16) : 0);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) v[i] = *reinterpret_cast<const u4*>(vals + off + 256 * i);
+            for (int i = 0; i < NV; ++i) v[i] = __builtin_nontemporal_load(reinterpret_cast<const u4*>(vals + off + 256 * i));
         };
 
         const int stop = tile0 + min(tiles, (split + 1) * per);
