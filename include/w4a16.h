@@ -221,8 +221,9 @@ int w4a16_kv4_read(const w4a16_kv4_cache* cache, const int64_t* slots, int64_t t
  * queries q_start[b] .. q_start[b + 1] - 1 are the last m of them: query i stands at
  * pos = seq_lens[b] - m + i and sees t < seq_lens[b], with `causal` only t <= pos, and with
  * window > 0 only t > pos - window.  Query head h reads KV head h / (heads / kv_heads).  A query that
- * sees nothing gives zeros (lse -inf); rows of q that belong to no sequence are not written.  Tokens on a table entry outside [0, pages) are not seen, and
- * lengths and starts are clamped to what the table and q hold, so no index reads out of bounds. */
+ * sees nothing gives zeros (lse -inf); rows of out and lse whose query belongs to no sequence are not
+ * written.  Tokens on a table entry outside [0, pages) are not seen, and lengths and starts are clamped
+ * to what the table and q hold, so no index reads out of bounds. */
 typedef struct w4a16_kv4_attention_args {
     const void* q;            /* fp16 or bf16 [tokens, heads, head_dim], head_dim contiguous */
     void*   out;              /* the same type, contiguous */

@@ -585,6 +585,37 @@ def test_other_streams_and_graphs(q_len, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [1, 40])
+def test_rows_of_no_sequence_are_not_written(lib, q_len):
+    """Queries before the first sequence's and past the last one's, with whatever the workspace held before."""
+    torch = torch_cuda()
+    P, H, D, G, n, before, after = 64, 2, 128, 128, 9000, 3, 7
+    g = torch.Generator(device="cuda").manual_seed(5)
+    cache = kv().kv4_cache(-(-n // P), P, H, D, G)
+    k, v = (torch.randn(n, H, D, device="cuda", generator=g).half() for _ in range(2))
+    kv().kv4_write(cache, k, v, torch.arange(n, device="cuda"), G)
+    q = torch.randn(before + q_len + after, 8, D, device="cuda", generator=g).half()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    table, lens = torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")[None], i32(n)
+    want, want_lse = kv().kv4_attention(q[before:before + q_len], cache, table, lens, G, q_start=i32(0, q_len), max_q=q_len, return_lse=True)
+    start, out, lse = i32(before, before + q_len), torch.full_like(q, 7), torch.full(q.shape[:2], 9.0, device="cuda")
+    c = Cache(cache.data_ptr(), cache.shape[0], P, H, D, G)
+    a = Args(q.data_ptr(), out.data_ptr(), lse.data_ptr(), q.stride(0), q.stride(1), q.shape[0], 8, 1, table.data_ptr(), table.shape[1],
+             table.stride(0), lens.data_ptr(), start.data_ptr(), q_len, 0, D**-0.5, 0, 1)
+    lim = (ctypes.c_int32 * 4)(256, 163840, 1024, 950)
+    size = lib.w4a16_kv4_attention_workspace(ctypes.byref(c), ctypes.byref(a), lim)
+    assert size > 0
+    workspace, counters = torch.full((size // 4 + 4,), 5, dtype=torch.int32, device="cuda"), torch.zeros(4096, dtype=torch.int32, device="cuda")
+    assert lib.w4a16_kv4_attention(ctypes.byref(c), ctypes.byref(a), lim, workspace.data_ptr(), size, counters.data_ptr(),
+                                   torch.cuda.current_stream().cuda_stream) == 0, lib.w4a16_last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(out[before:-after], want) and torch.equal(lse[before:-after], want_lse)
+    for rows in (slice(0, before), slice(before + q_len, None)):
+        assert (out[rows] == 7).all() and (lse[rows] == 9).all()
+    assert (counters == 0).all()
+
+
+@pytest.mark.gpu
 def test_empty_calls():
     torch = torch_cuda()
     c = kv().kv4_cache(2, 16, 2, 128, 64)

@@ -1051,13 +1051,16 @@ kv4_prompt_kernel(Kv4Attn a, int row_tiles, int splits, uint32_t page_magic, int
 // workgroup per row with the shares' sums through LDS took 17.6.
 template <int D>
 __global__ void __launch_bounds__(256)
-kv4_join_kernel(Kv4Attn a, int64_t rows, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml,
+kv4_join_kernel(Kv4Attn a, int64_t rows, int batch, int splits, const int* __restrict__ used, const float2* __restrict__ part_ml,
                 const float* __restrict__ part_o) {
     const int lane = threadIdx.x & 63;
     const int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row >= rows) return;
+    // nobody wrote used[row] of a query before the first sequence's or past the last one's
+    const int query = (int)((uint32_t)row / (uint32_t)a.heads);
+    const int from = a.q_start ? a.q_start[0] : 0, to = a.q_start ? a.q_start[batch] : a.tokens;
     const int parts = __builtin_amdgcn_readfirstlane(min(used[row], splits));
-    if (parts <= 1) return;
+    if (parts <= 1 || query < from || query >= to) return;
     const float2* const ml = part_ml + row * splits;
     const float* const o = part_o + row * splits * D + 2 * lane % D;
     float top = -INFINITY;
@@ -1230,7 +1233,7 @@ extern "C" int w4a16_kv4_attention(const w4a16_kv4_cache* cache, const w4a16_kv4
             if (plan.waves == 4) on(kv4_prompt_kernel<d.value, g.value, 4>);
             if (plan.splits > 1)
                 hipLaunchKernelGGL((kv4_join_kernel<d.value>), dim3((unsigned)((args->tokens * args->heads + 3) / 4)), dim3(256), 0, st, a,
-                                   args->tokens * args->heads, plan.splits, used, ml, po);
+                                   args->tokens * args->heads, (int)args->batch, plan.splits, used, ml, po);
         }
     });
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return kv4_fail(W4A16_ERR_HIP, "kv4_attention", hipGetErrorString(e));
