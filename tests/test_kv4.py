@@ -616,6 +616,43 @@ def test_rows_of_no_sequence_are_not_written(lib, q_len):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_len", [1, 40, 200])
+def test_a_table_much_wider_than_its_sequences(q_len):
+    """A table for the longest context that a server allows, 2^26 tokens here, and short sequences."""
+    torch_cuda()
+    rng = np.random.default_rng(q_len)
+    lens, P, H, D, G = [300, 201], 64, 8, 128, 128
+    cache, table = filled(rng, lens, P, H, D, G)
+    wide = np.full((2, (1 << 26) // P), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    q = values(rng, (2 * q_len, 32, D), torch.float16)
+    out, lse, ref = attend(q, cache, wide, lens, G, P, [0, q_len, 2 * q_len], max_q=q_len)
+    check(out, lse, ref, torch.float16)
+
+
+@pytest.mark.gpu
+def test_attention_of_a_long_prompt():
+    """132001 tokens with themselves, 32 heads on 8: rows here and there against 64 bits."""
+    torch = torch_cuda()
+    n, P, H, D, G = 132001, 64, 8, 64, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    cache = kv().kv4_cache(-(-n // P), P, H, D, G)
+    k, v = (torch.randn(n, H, D, device="cuda", generator=g).half() for _ in range(2))
+    slots = torch.arange(n, device="cuda")
+    kv().kv4_write(cache, k, v, slots, G)
+    q = torch.randn(n, 32, D, device="cuda", generator=g).half()
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device="cuda")  # noqa: E731
+    out = kv().kv4_attention(q, cache, torch.arange(cache.shape[0], dtype=torch.int32, device="cuda")[None], i32(n), G, q_start=i32(0, n), max_q=n)
+    hk, hv = (x.double() for x in kv().kv4_read(cache, slots, D, G, torch.float16))
+    for i in (0, 1, 63, 64, 4099, 65535, 65536, 131071, 131072, n - 1):
+        for h in (0, 13, 31):
+            p = (hk[:i + 1, h // 4] @ q[i, h].double() * D**-0.5).softmax(0)
+            want, spread = p @ hv[:i + 1, h // 4], p @ hv[:i + 1, h // 4].abs()
+            # the values were read back rounded to fp16: 2^-11 of each more, in keys as in values
+            check(out[i, h], None, (want.cpu().numpy(), None, 2 * spread.cpu().numpy()), torch.float16)
+
+
+@pytest.mark.gpu
 def test_empty_calls():
     torch = torch_cuda()
     c = kv().kv4_cache(2, 16, 2, 128, 64)

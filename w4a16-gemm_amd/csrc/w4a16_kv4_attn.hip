@@ -1096,8 +1096,8 @@ static const char* check_attention(const w4a16_kv4_cache* c, const w4a16_kv4_att
         a->batch >= 65536 || a->table_width * c->page_size >= (int64_t)1 << 27 || a->max_q < 1 || a->window < 0 ||
         a->tokens * a->heads >= (int64_t)1 << 31 || a->batch * a->heads >= (int64_t)1 << 31)
         return "dimensions out of range";
-    if ((a->tokens * (a->heads / c->kv_heads) / 4 + a->batch) * c->kv_heads >= ((int64_t)1 << 31) / std::max<int64_t>(1, a->table_width * c->page_size / 64 + 1))
-        return "too many queries times keys";
+    if (a->batch * (a->table_width * c->page_size / 64 + 1) >= (int64_t)1 << 31)     // all sequences' tiles are summed in 32 bits
+        return "too many sequences times keys";
     if (a->heads % c->kv_heads != 0) return "the query heads must be a multiple of the KV heads";
     if (!a->q_start && a->tokens != a->batch) return "without q_start there is one query per sequence";
     if (!(a->scale > 0.f) || !isfinite(a->scale)) return "scale must be positive and finite";
